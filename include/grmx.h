@@ -48,6 +48,11 @@ extern "C" {
 #define GRMX_FUSE_CONTRIB 1   /* out[B,Q,H]    = sum_r gate_r M[idx_r] q            */
 #define GRMX_FUSE_RESIDUAL_LN 2 /* out[B,Q,H]  = LayerNorm(h + sum_r gate_r M[idx_r] q) */
 
+/* reduction of grmx_linear_xent_fwd over the tokens */
+#define GRMX_REDUCE_NONE 0
+#define GRMX_REDUCE_SUM 1
+#define GRMX_REDUCE_MEAN 2 /* over the tokens that count; none: 0 / 0 */
+
 typedef struct grmx_device_info {
   int32_t device;
   int32_t cc_major;
@@ -417,8 +422,83 @@ int grmx_archive_push(const float* memory, float* archive, void* archive_bf16, i
                       int64_t slot, int64_t row_elems, void* stream);
 
 /*
+ * Softmax cross entropy of a vocabulary projection whose scores are never kept:
+ *
+ *   y[i,j] = hidden[i,:] . weight[j,:] + bias[j]        loss[i] = log(sum_j exp(y[i,j])) - y[i,targets[i]]
+ *
+ * hidden [N,D] and weight [V,D] in `dtype` (GRMX_BF16 or GRMX_F32), bias [V] in bias_dtype or NULL, targets
+ * int64 [N].  A token whose target equals ignore_index has loss 0 and no gradient; any other target outside
+ * [0,V) is treated the same and also sets bit 2 of the device error word.  loss is float32 [N]
+ * (GRMX_REDUCE_NONE) or [1] (sum, or mean over the tokens that count).  row_stats float32 [2,N] (maximum and
+ * sum of the scores' exponentials, base 2) and inv_count float32 [1] are what the backward call needs.
+ * bf16 products are exact and accumulate in fp32; fp32 inputs are split into three bf16 parts each, of which
+ * the six products above 2^-24 are taken.  Masked words (bias -inf) have probability 0; a row without any
+ * finite score gives NaN, as does a score of +inf or NaN.
+ *
+ * workspace: device memory of grmx_linear_xent_workspace(N, D, V, dtype, backward) bytes (0 if N == 0, -1 for
+ * sizes or a dtype that are refused), 256-byte aligned, contents irrelevant, not shared between calls that may
+ * run at the same time.
+ *
+ * The reference computes this as output_layer (grm/utils/train.py:223) followed by torch's cross entropy.
+ */
+int64_t grmx_linear_xent_workspace(int64_t N, int64_t D, int64_t V, int dtype, int backward);
+int grmx_linear_xent_fwd(const void* hidden, const void* weight, const void* bias, const int64_t* targets,
+                         int64_t ignore_index, float* loss, float* row_stats, float* inv_count, int64_t N,
+                         int64_t D, int64_t V, int dtype, int bias_dtype, int reduction, void* workspace,
+                         int64_t workspace_bytes, void* stream);
+
+/*
+ * Gradients of grmx_linear_xent_fwd: grad_loss float32 [N] (GRMX_REDUCE_NONE) or [1]; grad_hidden [N,D] and
+ * grad_weight [V,D] in `dtype`, grad_bias [V] in bias_dtype, each of which may be NULL (not wanted).  The scores
+ * are computed a second time, in pieces of the vocabulary whose gradients take at most 1 GiB of the workspace
+ * (more only where 256 words of all tokens do).  Sums are taken in a fixed order: the same call gives the same
+ * bits.  Every element of the outputs is written.
+ */
+int grmx_linear_xent_bwd(const float* grad_loss, const void* hidden, const void* weight, const void* bias,
+                         const int64_t* targets, int64_t ignore_index, const float* row_stats,
+                         const float* inv_count, void* grad_hidden, void* grad_weight, void* grad_bias, int64_t N,
+                         int64_t D, int64_t V, int dtype, int bias_dtype, int reduction, void* workspace,
+                         int64_t workspace_bytes, void* stream);
+
+/*
+ * The mixing rule after a block and its LayerNorm in one pass over rows of H values:
+ *
+ *   u = scale * update
+ *   s = online + u                             (gate NULL: residual rule)
+ *   s = G online + (1 - G) u, G = sigmoid(gate)     (gate rule)
+ *   out = (s - mean(s)) * rstd(s) * ln_weight + ln_bias,   rstd = 1 / sqrt(var(s) + eps)
+ *
+ * online, update, gate, out, sum_out [rows,H] in `dtype` (GRMX_F32 or GRMX_BF16); scale, ln_weight, ln_bias [H]
+ * in param_dtype (GRMX_F32, or dtype), each NULL for the identity; sum_out (s itself, rounded once) may be NULL.
+ * row_stats float32 [rows,2] (mean and rstd, what the backward call needs) may be NULL.  H <= 8192; arithmetic in
+ * fp32.  Rows and parameters on 16-byte boundaries move in 16-byte pieces, others value by value.
+ * out may not overlap the inputs.
+ *
+ * Replaces the residual and gate rules of RetrievedStateFusion with its LayerNorm (grm/core/aggregator.py:116-145)
+ * and the residual block between layers (grm/core/multilayer_grm.py:93,96) where they are trained;
+ * grmx_add_layer_norm is the plain sum, inference only.
+ */
+int grmx_fuse_norm_fwd(const void* online, const void* update, const void* gate, const void* scale,
+                       const void* ln_weight, const void* ln_bias, float eps, void* out, void* sum_out,
+                       float* row_stats, int64_t rows, int64_t H, int dtype, int param_dtype, void* stream);
+
+/*
+ * Gradients of grmx_fuse_norm_fwd.  grad_out and grad_sum [rows,H] in `dtype`: the gradients of out and sum_out,
+ * either NULL for zero, not both.  grad_online, grad_update, grad_gate [rows,H] in `dtype`, grad_scale,
+ * grad_weight, grad_bias [H] in param_dtype: each NULL if not wanted.  Column sums are taken in a fixed order.
+ * workspace: grmx_fuse_norm_workspace(rows, H) bytes (-1: refused sizes), 16-byte aligned, may be NULL if none of
+ * the three column sums is wanted.
+ */
+int64_t grmx_fuse_norm_workspace(int64_t rows, int64_t H);
+int grmx_fuse_norm_bwd(const void* grad_out, const void* grad_sum, const void* online, const void* update,
+                       const void* gate, const void* scale, const void* ln_weight, const float* row_stats,
+                       void* grad_online, void* grad_update, void* grad_gate, void* grad_scale, void* grad_weight,
+                       void* grad_bias, int64_t rows, int64_t H, int dtype, int param_dtype, void* workspace,
+                       int64_t workspace_bytes, void* stream);
+
+/*
  * Device error word: bit 0 = gather index out of range, bit 1 = a bounded
- * wait inside a kernel gave up.  grmx_device_error_word copies the word of
+ * wait inside a kernel gave up, bit 2 = a target outside the vocabulary.  grmx_device_error_word copies the word of
  * the current device to *out (synchronises that stream); reset clears it.
  */
 int grmx_device_error_word(uint32_t* out, void* stream);

@@ -48,6 +48,8 @@ CUDA_SOURCES = [
     "archive_push.cu",
     "normalize_rows.cu",
     "project_normalize.cu",
+    "linear_cross_entropy.cu",
+    "fuse_norm.cu",
 ]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -18,6 +18,7 @@ LIB_PATH = Path(__file__).resolve().parent / "libgrmx.so"
 F32, BF16, F16 = 0, 1, 2
 PATH_AUTO, PATH_FFMA, PATH_TCGEN05 = 0, 1, 2
 FUSE_RETRIEVED, FUSE_CONTRIB, FUSE_RESIDUAL_LN = 0, 1, 2
+REDUCE_NONE, REDUCE_SUM, REDUCE_MEAN = 0, 1, 2
 
 
 class DeviceInfo(ctypes.Structure):
@@ -102,6 +103,21 @@ SIGNATURES = {
     "grmx_normalize_rows": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_float, c_int, c_int, c_void_p]),
     "grmx_project_normalize": (c_int, [c_void_p] * 5 + [c_int64] * 3 + [c_float, c_void_p]),
     "grmx_archive_push": (c_int, [c_void_p] * 3 + [c_int64] * 4 + [c_void_p]),
+    "grmx_linear_xent_workspace": (c_int64, [c_int64] * 3 + [c_int, c_int]),
+    "grmx_linear_xent_fwd": (
+        c_int,
+        [c_void_p] * 4 + [c_int64] + [c_void_p] * 3 + [c_int64] * 3 + [c_int] * 3 + [c_void_p, c_int64, c_void_p],
+    ),
+    "grmx_linear_xent_bwd": (
+        c_int,
+        [c_void_p] * 5 + [c_int64] + [c_void_p] * 5 + [c_int64] * 3 + [c_int] * 3 + [c_void_p, c_int64, c_void_p],
+    ),
+    "grmx_fuse_norm_workspace": (c_int64, [c_int64, c_int64]),
+    "grmx_fuse_norm_fwd": (c_int, [c_void_p] * 6 + [c_float] + [c_void_p] * 3 + [c_int64, c_int64, c_int, c_int, c_void_p]),
+    "grmx_fuse_norm_bwd": (
+        c_int,
+        [c_void_p] * 14 + [c_int64, c_int64, c_int, c_int, c_void_p, c_int64, c_void_p],
+    ),
     "grmx_device_error_word": (c_int, [POINTER(c_uint32), c_void_p]),
     "grmx_device_error_reset": (c_int, [c_void_p]),
     "grmx_selftest_bounded_wait": (c_int, [c_uint32, c_void_p]),

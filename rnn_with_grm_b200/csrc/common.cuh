@@ -61,5 +61,6 @@ inline bool dtype_valid(int dtype) {
 
 constexpr uint32_t kErrGatherIndex = 1u;
 constexpr uint32_t kErrBoundedWait = 2u;
+constexpr uint32_t kErrTarget = 4u;
 
 }  // namespace grmx

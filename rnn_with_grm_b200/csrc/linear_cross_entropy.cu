@@ -1,0 +1,638 @@
+// Softmax cross entropy of a vocabulary projection, with its gradient, without keeping the scores.
+//
+//   y_ij = x_i . W_j + b_j     lse_i = log sum_j exp(y_ij)     loss_i = lse_i - y_{i,t_i}
+//   d_ij = g_i (exp(y_ij - lse_i) - [j = t_i])     dx = d W     dW = d^T x     db_j = sum_i d_ij
+//
+// Forward: one product x W^T whose epilogue reduces every 256-column tile of scores to a maximum and a sum
+// per row (base 2), and one small kernel that joins the tiles' pairs and adds the rows up.  Backward: the
+// vocabulary in pieces; for each piece the scores once more, their epilogue writing d (bf16, or three bf16
+// planes in full precision) to a workspace, then the two products that read it.  8 N V D FLOP in all, of
+// which 2 N V D are the scores computed a second time because they are not kept.
+//
+// Bound by the tensor cores at training sizes, by the stream of W where a few tokens are scored.
+// The maximum and the sum are kept apart (never as one log-sum-exp): exp(y - max) / sum then carries no
+// rounding of a sum that is as large as the scores, and a target that is the maximum itself leaves exactly
+// log(sum) as its loss.
+#include <cuda.h>
+
+#include <cstring>
+#include <mutex>
+
+#include "pair_gemm.cuh"
+
+namespace grmx {
+namespace {
+
+using namespace pair;
+
+constexpr float kLn2 = 0.6931471805599453f;
+
+inline int64_t round_up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// ------------------------------------------------------------------ operands as bf16 planes
+
+// [rows, cols] fp32 or bf16 -> planes of bf16 whose sum is the value (one plane for bf16: a copy with a pitch
+// that a tensor map can take).  x = h + m + l with h = bf16(x), m = bf16(x - h), l = bf16(x - h - m): 24 bits.
+// Values that are not finite stay whole in the first plane.
+template <typename T, int PLANES>
+__global__ void __launch_bounds__(256) planes_kernel(const T* __restrict__ src, __nv_bfloat16* __restrict__ dst, int64_t rows,
+                                                     int cols, int ld, int64_t plane_stride) {
+  const int64_t pairs = ld / 2;
+  const int64_t total = rows * pairs;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t r = i / pairs;
+    const int c = static_cast<int>(i - r * pairs) * 2;
+    float v[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) v[e] = c + e < cols ? to_float<T>(src[r * cols + c + e]) : 0.0f;
+#pragma unroll
+    for (int pl = 0; pl < PLANES; ++pl) {
+      __nv_bfloat162 b;
+      b.x = __float2bfloat16_rn(v[0]);
+      b.y = __float2bfloat16_rn(v[1]);
+      *reinterpret_cast<__nv_bfloat162*>(dst + pl * plane_stride + r * ld + c) = b;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float rest = v[e] - __bfloat162float(e == 0 ? b.x : b.y);
+        v[e] = isfinite(rest) ? rest : 0.0f;
+      }
+    }
+  }
+}
+
+struct Operand {
+  const void* ptr;
+  int64_t ld, plane_stride;
+  int planes;
+};
+
+bool readable_in_place(const void* ptr, int64_t cols, int dtype) {
+  return dtype == GRMX_BF16 && cols % 8 == 0 && (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0;
+}
+// By the width alone: a workspace is sized before the pointers are known, and has room for the copy of a
+// misaligned matrix too.
+int64_t operand_bytes(int64_t rows, int64_t cols, int dtype) {
+  return (dtype == GRMX_F32 ? 3 : 1) * round_up(rows * round_up(cols, 8) * 2, 256);
+}
+
+int make_operand(Operand* out, const void* src, int64_t rows, int64_t cols, int dtype, uint8_t** ws, cudaStream_t s) {
+  const int64_t bytes = operand_bytes(rows, cols, dtype);
+  uint8_t* dst = *ws;
+  *ws += bytes;
+  if (readable_in_place(src, cols, dtype)) {
+    *out = Operand{src, cols, rows * cols, 1};
+    return GRMX_OK;
+  }
+  const int64_t ld = round_up(cols, 8);
+  const int planes = dtype == GRMX_F32 ? 3 : 1;
+  const int64_t stride = bytes / planes / 2;
+  const int64_t blocks = ceil_div(rows * (ld / 2), 256);
+  const unsigned grid = static_cast<unsigned>(blocks < 148 * 16 ? blocks : 148 * 16);
+  __nv_bfloat16* d = reinterpret_cast<__nv_bfloat16*>(dst);
+  if (dtype == GRMX_F32) {
+    planes_kernel<float, 3><<<grid, 256, 0, s>>>(static_cast<const float*>(src), d, rows, static_cast<int>(cols),
+                                                  static_cast<int>(ld), stride);
+  } else {
+    planes_kernel<__nv_bfloat16, 1><<<grid, 256, 0, s>>>(static_cast<const __nv_bfloat16*>(src), d, rows,
+                                                          static_cast<int>(cols), static_cast<int>(ld), stride);
+  }
+  *out = Operand{dst, ld, stride, planes};
+  return check_launch("loss operand planes");
+}
+
+// ------------------------------------------------------------------ joining the tiles' maxima and sums
+
+constexpr int kJoinRows = 32;
+constexpr int kJoinSlices = 8;
+
+// partials [parts][rows] -> maximum, sum and loss per row; with a reduction, the blocks' sums are added up by
+// the block that finishes last, always in the same order.
+__global__ void __launch_bounds__(kJoinRows * kJoinSlices)
+loss_join_kernel(const float2* __restrict__ partials, const float* __restrict__ target_score,
+                 const int64_t* __restrict__ targets, int64_t ignore_index, int64_t vocab, int64_t rows, int parts,
+                 int reduction, float* __restrict__ row_max, float* __restrict__ row_sum, float* __restrict__ loss,
+                 float* __restrict__ inv_count, double* __restrict__ block_loss, int* __restrict__ block_count,
+                 uint32_t* ticket, uint32_t* error_word) {
+  __shared__ float2 s_part[kJoinSlices][kJoinRows];
+  __shared__ double s_loss[kJoinRows * kJoinSlices];
+  __shared__ int s_count[kJoinRows * kJoinSlices];
+  __shared__ bool s_last;
+  const int r = threadIdx.x % kJoinRows, slice = threadIdx.x / kJoinRows;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kJoinRows + r;
+  float mx = -INFINITY, sum = 0.0f;
+  if (row < rows) {
+    for (int i = slice; i < parts; i += kJoinSlices) {
+      const float2 q = partials[static_cast<int64_t>(i) * rows + row];
+      const float next = fmaxf(mx, q.x);
+      const float base = next == -INFINITY ? 0.0f : next;
+      sum = sum * exp2_fast(mx - base) + q.y * exp2_fast(q.x - base);
+      mx = next;
+    }
+  }
+  s_part[slice][r] = make_float2(mx, sum);
+  __syncthreads();
+  float value = 0.0f;
+  int counted = 0;
+  if (slice == 0 && row < rows) {
+    for (int i = 1; i < kJoinSlices; ++i) {
+      const float2 q = s_part[i][r];
+      const float next = fmaxf(mx, q.x);
+      const float base = next == -INFINITY ? 0.0f : next;
+      sum = sum * exp2_fast(mx - base) + q.y * exp2_fast(q.x - base);
+      mx = next;
+    }
+    if (mx == -INFINITY) sum = __int_as_float(0x7fc00000);    // every word masked: no distribution
+    row_max[row] = mx;
+    row_sum[row] = sum;
+    const int64_t t = targets[row];
+    if (t != ignore_index) {
+      if (t >= 0 && t < vocab) {
+        value = ((mx - target_score[row]) + log2f(sum)) * kLn2;
+        counted = 1;
+      } else if (error_word != nullptr) {
+        atomicOr(error_word, kErrTarget);
+      }
+    }
+    if (reduction == GRMX_REDUCE_NONE) loss[row] = value;
+  }
+  if (reduction == GRMX_REDUCE_NONE) return;
+  if (slice == 0) {
+    double v = value;
+    int n = counted;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      v += __shfl_xor_sync(0xffffffffu, v, o);
+      n += __shfl_xor_sync(0xffffffffu, n, o);
+    }
+    if (r == 0) {
+      block_loss[blockIdx.x] = v;
+      block_count[blockIdx.x] = n;
+      __threadfence();
+      s_last = atomicAdd(ticket, 1u) == gridDim.x - 1;
+    }
+  }
+  __syncthreads();
+  if (!s_last) return;
+  __threadfence();
+  double v = 0.0;
+  int n = 0;
+  for (unsigned i = threadIdx.x; i < gridDim.x; i += kJoinRows * kJoinSlices) {
+    v += __ldcg(block_loss + i);
+    n += __ldcg(block_count + i);
+  }
+  s_loss[threadIdx.x] = v;
+  s_count[threadIdx.x] = n;
+  __syncthreads();
+  for (int o = kJoinRows * kJoinSlices / 2; o > 0; o >>= 1) {
+    if (threadIdx.x < o) {
+      s_loss[threadIdx.x] += s_loss[threadIdx.x + o];
+      s_count[threadIdx.x] += s_count[threadIdx.x + o];
+    }
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) {
+    const double count = s_count[0];
+    // no token counts: the mean is 0 / 0, as of an empty list, and no row has a gradient
+    *loss = static_cast<float>(reduction == GRMX_REDUCE_MEAN ? s_loss[0] / count : s_loss[0]);
+    *inv_count = reduction == GRMX_REDUCE_MEAN ? (count > 0.0 ? static_cast<float>(1.0 / count) : 0.0f) : 1.0f;
+  }
+}
+
+// ------------------------------------------------------------------ sums of partial results
+
+// out[r, c] = sum over s of part[s][r][c]   (part pitch ld, out dense), VEC columns per thread
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256) sum_splits_kernel(const float* __restrict__ part, T* __restrict__ out, int64_t rows,
+                                                         int cols, int ld, int64_t split_stride, int splits) {
+  const int per_row = cols / VEC;
+  const int64_t total = rows * per_row;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t r = i / per_row;
+    const int c = static_cast<int>(i - r * per_row) * VEC;
+    const float* src = part + r * ld + c;
+    float v[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] = 0.0f;
+    for (int s = 0; s < splits; ++s) {
+      if (VEC == 4) {
+        const float4 q = __ldcs(reinterpret_cast<const float4*>(src + s * split_stride));
+        v[0] += q.x;
+        if (VEC > 1) { v[1 % VEC] += q.y; v[2 % VEC] += q.z; v[3 % VEC] += q.w; }
+      } else {
+        v[0] += src[s * split_stride];
+      }
+    }
+    if (VEC == 4 && sizeof(T) == 2) {
+      *reinterpret_cast<uint2*>(out + r * cols + c) = make_uint2(pack_bf16(v[0], v[1 % VEC]), pack_bf16(v[2 % VEC], v[3 % VEC]));
+    } else if (VEC == 4) {
+      *reinterpret_cast<float4*>(out + r * cols + c) = make_float4(v[0], v[1 % VEC], v[2 % VEC], v[3 % VEC]);
+    } else {
+      out[r * cols + c] = from_float<T>(v[0]);
+    }
+  }
+}
+
+int launch_sum_splits(const float* part, void* out, int64_t rows, int64_t cols, int64_t ld, int64_t split_stride, int splits,
+                      int dtype, cudaStream_t s) {
+  const bool vec = cols % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 15u) == 0;
+  const int64_t blocks = ceil_div(rows * cols, vec ? 1024 : 256);
+  const unsigned grid = static_cast<unsigned>(blocks < 148 * 16 ? blocks : 148 * 16);
+  const int c = static_cast<int>(cols), l = static_cast<int>(ld);
+  if (dtype == GRMX_F32) {
+    if (vec) sum_splits_kernel<float, 4><<<grid, 256, 0, s>>>(part, static_cast<float*>(out), rows, c, l, split_stride, splits);
+    else sum_splits_kernel<float, 1><<<grid, 256, 0, s>>>(part, static_cast<float*>(out), rows, c, l, split_stride, splits);
+  } else {
+    __nv_bfloat16* o = static_cast<__nv_bfloat16*>(out);
+    if (vec) sum_splits_kernel<__nv_bfloat16, 4><<<grid, 256, 0, s>>>(part, o, rows, c, l, split_stride, splits);
+    else sum_splits_kernel<__nv_bfloat16, 1><<<grid, 256, 0, s>>>(part, o, rows, c, l, split_stride, splits);
+  }
+  return check_launch("loss split sums");
+}
+
+// db[v0 + c] = sum over the blocks of 32 token rows; 32 columns x 8 slices per block, slices joined in order
+template <typename T>
+__global__ void __launch_bounds__(256) bias_sum_kernel(const float* __restrict__ partials, int64_t blocks, int64_t pitch,
+                                                       int64_t cols, const float* scale, const float* scale2,
+                                                       T* __restrict__ out) {
+  __shared__ float s_sum[8][32];
+  const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
+  const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;
+  float sum = 0.0f;
+  for (int64_t b = slice; b < blocks; b += 8) sum += partials[b * pitch + c];   // the pitch covers whole tiles
+  s_sum[slice][lane] = sum;
+  __syncthreads();
+  if (slice == 0 && c < cols) {
+    for (int i = 1; i < 8; ++i) sum += s_sum[i][lane];
+    if (scale != nullptr) sum *= *scale;
+    if (scale2 != nullptr) sum *= *scale2;
+    out[c] = from_float<T>(sum);
+  }
+}
+
+// ------------------------------------------------------------------ launches
+
+int pairs_on_device() {
+  static std::mutex mutex;
+  static int cached[64] = {0};
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return 74;
+  std::lock_guard<std::mutex> lock(mutex);
+  if (cached[device] == 0) {
+    int sms = 0;
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || sms < 2) sms = 148;
+    cached[device] = sms / 2;
+  }
+  return cached[device];
+}
+
+template <int EPI, bool A_MN, bool B_MN, bool SEG>
+int launch_pair(const Maps& maps, const Params& p, const char* what, cudaStream_t s) {
+  auto kernel = pair_gemm_kernel<EPI, A_MN, B_MN, SEG>;
+  static std::mutex mutex;
+  static bool configured[64] = {false};
+  int device = 0;
+  cudaGetDevice(&device);
+  {
+    std::lock_guard<std::mutex> lock(mutex);
+    if (device < 0 || device >= 64 || !configured[device]) {
+      const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemAlloc);
+      if (e != cudaSuccess) {
+        cudaGetLastError();
+        return fail(GRMX_ERR_LAUNCH, "%s: cannot reserve %d bytes of shared memory: %s", what, kSmemAlloc, cudaGetErrorString(e));
+      }
+      if (device >= 0 && device < 64) configured[device] = true;
+    }
+  }
+  const int64_t units = static_cast<int64_t>(p.m_tiles) * p.n_tiles * p.splits;
+  const int pairs = pairs_on_device();
+  const unsigned grid = 2u * static_cast<unsigned>(units < pairs ? units : pairs);
+  kernel<<<grid, kThreads, kSmemAlloc, s>>>(maps, p, device_error_word_ptr());
+  return check_launch(what);
+}
+
+// A K-major operand tile is one box of 64 k x 128 rows; an MN-major one is two boxes of 64 columns x 64 k.
+bool operand_map(CUtensorMap* map, const Operand& o, int64_t rows, int64_t cols, bool mn_major) {
+  return make_matrix_map(map, o.ptr, false, o.planes, rows, cols, o.ld, o.plane_stride, 64, mn_major ? 64 : 128);
+}
+
+// How many parts the contraction of an [m_tiles x n_tiles] result is cut into so that the pairs are busy to the
+// end: waves of blocks (0.29 us per 256 x 256 x 64 block and plane product, measured) against writing and
+// reading one more fp32 copy of the result (about 5 TB/s).
+int choose_splits(int64_t tiles, int64_t k_blocks, int64_t result_elems, int products, int pairs) {
+  int best = 1;
+  double best_cost = 1e30;
+  const int64_t most = k_blocks < 64 ? k_blocks : 64;
+  for (int64_t s = 1; s <= most; ++s) {
+    const int64_t per = ceil_div(k_blocks, s);
+    if (ceil_div(k_blocks, per) != s) continue;
+    const double cost = ceil_div(tiles * s, pairs) * (per * products * 0.29 + 2.0) + (s > 1 ? s * result_elems * 8.0 / 5e6 + 3.0 : 0.0);
+    if (cost < best_cost * 0.97) {
+      best_cost = cost;
+      best = static_cast<int>(s);
+    }
+  }
+  return best;
+}
+
+// The plan of a backward pass and the layout of its workspace: a function of the sizes alone.
+struct BackwardPlan {
+  int64_t piece;               // words per piece, a multiple of 256
+  int pieces;
+  int splits_x, splits_w;
+  int64_t pitch;               // of the fp32 partial results
+  int64_t off_x, off_w, off_d, off_dx, off_dw, off_bias, bytes;
+};
+
+constexpr int64_t kPieceBytes = int64_t(1) << 30;            // most of the gradient of the scores that is held at a time
+
+BackwardPlan plan_backward(int64_t N, int64_t D, int64_t V, int dtype, int pairs) {
+  BackwardPlan b;
+  const int planes = dtype == GRMX_F32 ? 3 : 1;
+  const int products = dtype == GRMX_F32 ? 6 : 1;
+  const int64_t whole = round_up(V, kTileN);
+  int64_t most = kPieceBytes / (2 * planes * N) / kTileN * kTileN;
+  if (most < kTileN) most = kTileN;
+  if (most > whole) most = whole;
+  b.pieces = static_cast<int>(ceil_div(whole, most));
+  b.piece = round_up(ceil_div(whole, b.pieces), kTileN);
+  b.pieces = static_cast<int>(ceil_div(whole, b.piece));
+  b.pitch = round_up(D, 8);
+  const int64_t nt = ceil_div(D, kTileN);
+  b.splits_x = choose_splits(ceil_div(N, kTileM) * nt, b.piece / kBlockK, N * D, products, pairs);
+  b.splits_w = choose_splits(b.piece / kTileM * nt, ceil_div(N, kBlockK), b.piece * D, products, pairs);
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t here = at;
+    at += round_up(bytes, 1024);
+    return here;
+  };
+  b.off_x = take(operand_bytes(N, D, dtype));
+  b.off_w = take(operand_bytes(V, D, dtype));
+  b.off_d = take(planes * N * b.piece * 2);
+  b.off_dx = take(b.splits_x * N * b.pitch * 4);
+  b.off_dw = take(b.splits_w * b.piece * b.pitch * 4);
+  b.off_bias = take(ceil_div(N, kTileM) * 8 * b.piece * 4);
+  b.bytes = at;
+  return b;
+}
+
+struct ForwardPlan {
+  int parts;
+  int64_t join_blocks;
+  int64_t off_x, off_w, off_part, off_target, off_loss, off_count, off_ticket, bytes;
+};
+
+ForwardPlan plan_forward(int64_t N, int64_t D, int64_t V, int dtype) {
+  ForwardPlan f;
+  f.parts = static_cast<int>(ceil_div(V, kTileN)) * (dtype == GRMX_F32 ? 2 : 1);
+  f.join_blocks = ceil_div(N, kJoinRows);
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t here = at;
+    at += round_up(bytes, 1024);
+    return here;
+  };
+  f.off_x = take(operand_bytes(N, D, dtype));
+  f.off_w = take(operand_bytes(V, D, dtype));
+  f.off_part = take(f.parts * N * 8);
+  f.off_target = take(N * 4);
+  f.off_loss = take(f.join_blocks * 8);
+  f.off_count = take(f.join_blocks * 4);
+  f.off_ticket = take(4);
+  f.bytes = at;
+  return f;
+}
+
+int check_sizes(const char* who, int64_t N, int64_t D, int64_t V, int dtype) {
+  GRMX_REQUIRE(dtype == GRMX_F32 || dtype == GRMX_BF16, "%s: dtype must be f32 or bf16", who);
+  GRMX_REQUIRE(N >= 0 && D > 0 && V > 0, "%s: bad sizes", who);
+  // tile coordinates and unit numbers are 32-bit
+  GRMX_REQUIRE(N <= (int64_t(1) << 28) && V <= (int64_t(1) << 28) && D <= (int64_t(1) << 20), "%s: sizes exceed the tile coordinates", who);
+  GRMX_REQUIRE(ceil_div(N, kTileM) * ceil_div(V, kTileN) <= 0x3fffffffLL, "%s: too many tiles", who);
+  return GRMX_OK;
+}
+
+int check_device(const char* who) {
+  if (!tc::device_is_sm100() || tc::encode_tiled_fn() == nullptr) {
+    return fail(GRMX_ERR_DEVICE, "%s: needs an sm_100 device with tensor-map support", who);
+  }
+  return GRMX_OK;
+}
+
+#define GRMX_TRY(call)                 \
+  do {                                 \
+    const int rc_ = (call);            \
+    if (rc_ != GRMX_OK) return rc_;    \
+  } while (0)
+
+}  // namespace
+}  // namespace grmx
+
+extern "C" int64_t grmx_linear_xent_workspace(int64_t N, int64_t D, int64_t V, int dtype, int backward) {
+  using namespace grmx;
+  if (check_sizes("grmx_linear_xent_workspace", N, D, V, dtype) != GRMX_OK) return -1;
+  if (N == 0) return 0;
+  return backward ? plan_backward(N, D, V, dtype, pairs_on_device()).bytes : plan_forward(N, D, V, dtype).bytes;
+}
+
+extern "C" int grmx_linear_xent_fwd(const void* hidden, const void* weight, const void* bias, const int64_t* targets,
+                                    int64_t ignore_index, float* loss, float* row_stats, float* inv_count, int64_t N,
+                                    int64_t D, int64_t V, int dtype, int bias_dtype, int reduction, void* workspace,
+                                    int64_t workspace_bytes, void* stream) {
+  using namespace grmx;
+  const char* who = "grmx_linear_xent_fwd";
+  GRMX_TRY(check_sizes(who, N, D, V, dtype));
+  GRMX_REQUIRE(reduction == GRMX_REDUCE_NONE || reduction == GRMX_REDUCE_SUM || reduction == GRMX_REDUCE_MEAN, "%s: bad reduction", who);
+  GRMX_REQUIRE(bias == nullptr || bias_dtype == GRMX_F32 || bias_dtype == GRMX_BF16, "%s: bias must be f32 or bf16", who);
+  GRMX_REQUIRE(N > 0, "%s: needs at least one token", who);
+  GRMX_REQUIRE(hidden && weight && targets && loss && row_stats && inv_count, "%s: NULL tensor pointer", who);
+  const ForwardPlan f = plan_forward(N, D, V, dtype);
+  GRMX_REQUIRE(workspace != nullptr && workspace_bytes >= f.bytes, "%s: workspace of %lld bytes, needs %lld", who,
+               (long long)workspace_bytes, (long long)f.bytes);
+  GRMX_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 255u) == 0, "%s: workspace must be 256-byte aligned", who);
+  GRMX_TRY(check_device(who));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  Operand x, w;
+  uint8_t* at = ws + f.off_x;
+  GRMX_TRY(make_operand(&x, hidden, N, D, dtype, &at, s));
+  at = ws + f.off_w;
+  GRMX_TRY(make_operand(&w, weight, V, D, dtype, &at, s));
+  Maps maps;
+  if (!operand_map(&maps.a, x, N, D, false) || !operand_map(&maps.b, w, V, D, false)) {
+    return fail(GRMX_ERR_LAUNCH, "%s: cuTensorMapEncodeTiled failed", who);
+  }
+  maps.c = maps.a;
+  Params p;
+  memset(&p, 0, sizeof(p));
+  p.m_tiles = static_cast<int>(ceil_div(N, kTileM));
+  p.n_tiles = static_cast<int>(ceil_div(V, kTileN));
+  p.splits = 1;
+  p.k_blocks = p.blocks_per_split = static_cast<int>(ceil_div(D, kBlockK));
+  p.rows = N;
+  p.cols = V;
+  p.vocab = V;
+  p.bias = bias;
+  p.bias_dtype = bias_dtype;
+  p.targets = targets;
+  p.ignore_index = ignore_index;
+  p.partials = reinterpret_cast<float2*>(ws + f.off_part);
+  p.target_score = reinterpret_cast<float*>(ws + f.off_target);
+  p.ticket = reinterpret_cast<uint32_t*>(ws + f.off_ticket);
+  GRMX_TRY(dtype == GRMX_F32 ? (launch_pair<kEpiLse, false, false, true>(maps, p, "loss scores", s))
+                             : (launch_pair<kEpiLse, false, false, false>(maps, p, "loss scores", s)));
+  loss_join_kernel<<<static_cast<unsigned>(f.join_blocks), kJoinRows * kJoinSlices, 0, s>>>(
+      p.partials, p.target_score, targets, ignore_index, V, N, f.parts, reduction, row_stats, row_stats + N, loss, inv_count,
+      reinterpret_cast<double*>(ws + f.off_loss), reinterpret_cast<int*>(ws + f.off_count), p.ticket, device_error_word_ptr());
+  return check_launch("loss join");
+}
+
+extern "C" int grmx_linear_xent_bwd(const float* grad_loss, const void* hidden, const void* weight, const void* bias,
+                                    const int64_t* targets, int64_t ignore_index, const float* row_stats,
+                                    const float* inv_count, void* grad_hidden, void* grad_weight, void* grad_bias, int64_t N,
+                                    int64_t D, int64_t V, int dtype, int bias_dtype, int reduction, void* workspace,
+                                    int64_t workspace_bytes, void* stream) {
+  using namespace grmx;
+  const char* who = "grmx_linear_xent_bwd";
+  GRMX_TRY(check_sizes(who, N, D, V, dtype));
+  GRMX_REQUIRE(reduction == GRMX_REDUCE_NONE || reduction == GRMX_REDUCE_SUM || reduction == GRMX_REDUCE_MEAN, "%s: bad reduction", who);
+  GRMX_REQUIRE((bias == nullptr && grad_bias == nullptr) || bias_dtype == GRMX_F32 || bias_dtype == GRMX_BF16,
+               "%s: bias must be f32 or bf16", who);
+  GRMX_REQUIRE(N > 0, "%s: needs at least one token", who);
+  if (!grad_hidden && !grad_weight && !grad_bias) return GRMX_OK;
+  GRMX_REQUIRE(grad_loss && hidden && weight && targets && row_stats && inv_count, "%s: NULL tensor pointer", who);
+  const int pairs = pairs_on_device();
+  const BackwardPlan b = plan_backward(N, D, V, dtype, pairs);
+  GRMX_REQUIRE(workspace != nullptr && workspace_bytes >= b.bytes, "%s: workspace of %lld bytes, needs %lld", who,
+               (long long)workspace_bytes, (long long)b.bytes);
+  GRMX_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 255u) == 0, "%s: workspace must be 256-byte aligned", who);
+  GRMX_TRY(check_device(who));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  const bool f32 = dtype == GRMX_F32;
+  const int planes = f32 ? 3 : 1;
+  const int64_t elem = f32 ? 4 : 2;
+  Operand x, w;
+  uint8_t* at = ws + b.off_x;
+  GRMX_TRY(make_operand(&x, hidden, N, D, dtype, &at, s));
+  at = ws + b.off_w;
+  GRMX_TRY(make_operand(&w, weight, V, D, dtype, &at, s));
+  const int n_tiles_d = static_cast<int>(ceil_div(D, kTileN));
+  float* part_x = reinterpret_cast<float*>(ws + b.off_dx);
+  float* part_w = reinterpret_cast<float*>(ws + b.off_dw);
+  float* part_b = reinterpret_cast<float*>(ws + b.off_bias);
+  // A factor that all tokens share (the upstream gradient of a sum or a mean, 1 / count) multiplies the finished
+  // sums: d is then p - [target] itself, and the -1 of a target, which carries most of the gradient, is exact in
+  // bf16 where p is small.  A factor per token has to go into d before it is rounded.
+  const float* scale = reduction == GRMX_REDUCE_NONE ? nullptr : grad_loss;
+  const float* scale2 = reduction == GRMX_REDUCE_MEAN ? inv_count : nullptr;
+  // a result that is complete after one product leaves its epilogue in the caller's type
+  auto storable = [&](const void* out) { return D * elem % 16 == 0 && (reinterpret_cast<uintptr_t>(out) & 15u) == 0; };
+  const bool direct_x = b.pieces == 1 && b.splits_x == 1 && storable(grad_hidden);
+  const bool direct_w = b.splits_w == 1 && storable(grad_weight);
+
+  for (int piece = 0; piece < b.pieces; ++piece) {
+    const int64_t v0 = piece * b.piece;
+    const int64_t words = V - v0 < b.piece ? V - v0 : b.piece;       // of the vocabulary in this piece
+    const int64_t width = round_up(words, kTileN);
+    const Operand d{ws + b.off_d, b.piece, N * b.piece, planes};
+    const Operand w_piece{static_cast<const uint8_t*>(w.ptr) + v0 * w.ld * 2, w.ld, w.plane_stride, w.planes};
+    {
+      Maps maps;
+      if (!operand_map(&maps.a, x, N, D, false) || !operand_map(&maps.b, w_piece, words, D, false) ||
+          !make_matrix_map(&maps.c, d.ptr, false, planes, N, width, d.ld, d.plane_stride, 64, 128)) {
+        return fail(GRMX_ERR_LAUNCH, "%s: cuTensorMapEncodeTiled failed", who);
+      }
+      Params p;
+      memset(&p, 0, sizeof(p));
+      p.m_tiles = static_cast<int>(ceil_div(N, kTileM));
+      p.n_tiles = static_cast<int>(width / kTileN);
+      p.splits = 1;
+      p.k_blocks = p.blocks_per_split = static_cast<int>(ceil_div(D, kBlockK));
+      p.rows = N;
+      p.cols = width;
+      p.v0 = v0;
+      p.vocab = V;
+      p.bias = bias;
+      p.bias_dtype = bias_dtype;
+      p.targets = targets;
+      p.ignore_index = ignore_index;
+      p.row_max = row_stats;
+      p.row_sum = row_stats + N;
+      p.grad = reduction == GRMX_REDUCE_NONE ? grad_loss : nullptr;
+      p.bias_partials = grad_bias != nullptr ? part_b : nullptr;
+      GRMX_TRY(f32 ? (launch_pair<kEpiGrad, false, false, true>(maps, p, "loss score gradient", s))
+                   : (launch_pair<kEpiGrad, false, false, false>(maps, p, "loss score gradient", s)));
+    }
+    if (grad_bias != nullptr) {
+      const int64_t blocks = ceil_div(N, kTileM) * 8;
+      const unsigned grid = static_cast<unsigned>(ceil_div(words, 32));
+      if (bias_dtype == GRMX_F32) {
+        bias_sum_kernel<float><<<grid, 256, 0, s>>>(part_b, blocks, width, words, scale, scale2, static_cast<float*>(grad_bias) + v0);
+      } else {
+        bias_sum_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(part_b, blocks, width, words, scale, scale2,
+                                                             static_cast<__nv_bfloat16*>(grad_bias) + v0);
+      }
+      GRMX_TRY(check_launch("loss bias gradient"));
+    }
+    if (grad_hidden != nullptr) {
+      // dx = d W: the words of the piece are the contraction; later pieces add to the first one's result
+      Maps maps;
+      const bool to_f32 = f32 || !direct_x;
+      const int64_t ld = direct_x ? D : b.pitch;
+      if (!operand_map(&maps.a, d, N, width, false) || !operand_map(&maps.b, w_piece, words, D, true) ||
+          !make_matrix_map(&maps.c, direct_x ? grad_hidden : part_x, to_f32, b.splits_x, N, D, ld, N * ld, to_f32 ? 32 : 64, 128)) {
+        return fail(GRMX_ERR_LAUNCH, "%s: cuTensorMapEncodeTiled failed", who);
+      }
+      Params p;
+      memset(&p, 0, sizeof(p));
+      p.m_tiles = static_cast<int>(ceil_div(N, kTileM));
+      p.n_tiles = n_tiles_d;
+      p.k_blocks = static_cast<int>(width / kBlockK);
+      p.blocks_per_split = static_cast<int>(ceil_div(b.piece / kBlockK, b.splits_x));
+      // a last piece that is narrower than the others has fewer parts; the ones that it leaves out keep their sums
+      p.splits = static_cast<int>(ceil_div(p.k_blocks, p.blocks_per_split));
+      p.rows = N;
+      p.cols = D;
+      p.store_f32 = to_f32;
+      p.store_add = piece > 0;
+      p.scale = scale;
+      p.scale2 = scale2;
+      GRMX_TRY(f32 ? (launch_pair<kEpiStore, false, true, true>(maps, p, "loss hidden gradient", s))
+                   : (launch_pair<kEpiStore, false, true, false>(maps, p, "loss hidden gradient", s)));
+    }
+    if (grad_weight != nullptr) {
+      // dW = d^T x: the tokens are the contraction
+      Maps maps;
+      const bool to_f32 = f32 || !direct_w;
+      const int64_t ld = direct_w ? D : b.pitch;
+      void* out = static_cast<uint8_t*>(grad_weight) + v0 * D * elem;
+      if (!operand_map(&maps.a, d, N, width, true) || !operand_map(&maps.b, x, N, D, true) ||
+          !make_matrix_map(&maps.c, direct_w ? out : part_w, to_f32, b.splits_w, words, D, ld, b.piece * ld, to_f32 ? 32 : 64, 128)) {
+        return fail(GRMX_ERR_LAUNCH, "%s: cuTensorMapEncodeTiled failed", who);
+      }
+      Params p;
+      memset(&p, 0, sizeof(p));
+      p.m_tiles = static_cast<int>(width / kTileM);
+      p.n_tiles = n_tiles_d;
+      p.k_blocks = static_cast<int>(ceil_div(N, kBlockK));
+      p.blocks_per_split = static_cast<int>(ceil_div(p.k_blocks, b.splits_w));
+      p.splits = b.splits_w;
+      p.rows = words;
+      p.cols = D;
+      p.store_f32 = to_f32;
+      p.scale = scale;
+      p.scale2 = scale2;
+      GRMX_TRY(f32 ? (launch_pair<kEpiStore, true, true, true>(maps, p, "loss weight gradient", s))
+                   : (launch_pair<kEpiStore, true, true, false>(maps, p, "loss weight gradient", s)));
+      if (!direct_w) {
+        GRMX_TRY(launch_sum_splits(part_w, out, words, D, b.pitch, b.piece * b.pitch, b.splits_w, dtype, s));
+      }
+    }
+  }
+  if (grad_hidden != nullptr && !direct_x) {
+    GRMX_TRY(launch_sum_splits(part_x, grad_hidden, N, D, b.pitch, N * b.pitch, b.splits_x, dtype, s));
+  }
+  return GRMX_OK;
+}

@@ -91,6 +91,29 @@ bool make_token_half_map(CUtensorMap* map, const void* base, int64_t B, int64_t 
   return encode_token_map(map, MapKey{base, B, T, D, 1});
 }
 
+bool make_matrix_map(CUtensorMap* map, const void* base, bool f32, int64_t planes, int64_t rows, int64_t cols, int64_t ld,
+                     int64_t plane_stride, int box_cols, int box_rows) {
+  EncodeTiledFn encode = encode_tiled_fn();
+  if (encode == nullptr) return false;
+  const cuuint64_t es = f32 ? 4 : 2;
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(planes)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(ld) * es, static_cast<cuuint64_t>(plane_stride) * es};
+  const cuuint32_t box[3] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows), 1};
+  const cuuint32_t elem_strides[3] = {1, 1, 1};
+  for (int attempt = 0; attempt < 2; ++attempt) {
+    if (encode(map, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims,
+               strides, box, elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS) {
+      return true;
+    }
+    // A driver call needs a current context, and a thread that has made no runtime call yet (autograd's own
+    // thread in its first backward pass) has none: setting its device binds the device's primary context.
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess || cudaSetDevice(device) != cudaSuccess) return false;
+  }
+  return false;
+}
+
 namespace {
 
 // Four warps wait on a barrier that nothing completes.  The first to run out of polls raises the

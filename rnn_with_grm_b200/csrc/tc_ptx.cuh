@@ -381,6 +381,11 @@ EncodeTiledFn encode_tiled_fn();
 bool make_token_map(CUtensorMap* map, const void* base, int64_t B, int64_t T, int64_t D);
 // the same tensor as a store target: box = 32 features x 128 tokens x 1 row, 64-byte swizzle
 bool make_token_half_map(CUtensorMap* map, const void* base, int64_t B, int64_t T, int64_t D);
+// 3-D map over planes of row-major matrices [planes][rows][cols] of bf16 or fp32 with a row pitch of `ld` elements
+// (a multiple of 16 bytes): box = box_cols x box_rows x 1, 128-byte swizzle (box_cols * element size = 128).
+// Encoded anew by every call.
+bool make_matrix_map(CUtensorMap* map, const void* base, bool f32, int64_t planes, int64_t rows, int64_t cols, int64_t ld,
+                     int64_t plane_stride, int box_cols, int box_rows);
 bool device_is_sm100();
 // one CTA that lets a bounded wait expire on purpose (see grmx_selftest_bounded_wait)
 int launch_bounded_wait_selftest(uint32_t limit, cudaStream_t stream);

@@ -10,6 +10,7 @@
 #include <torch/extension.h>
 
 #include <atomic>
+#include <cmath>
 #include <tuple>
 
 #include "grmx.h"
@@ -548,6 +549,226 @@ at::Tensor retrieve_fuse_tc_cuda(const at::Tensor& archive, const at::Tensor& in
   return out;
 }
 
+// ---- vocabulary loss: hidden [N,D] and weight [V,D] (bf16 or fp32), targets int64 [N], bias [V]? ----
+
+struct LossArgs {
+  at::Tensor hidden, weight, targets, bias;
+  int64_t N, D, V;
+  int dtype, bias_dtype;
+};
+
+LossArgs check_loss_inputs(const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& targets,
+                           const c10::optional<at::Tensor>& bias, int64_t reduction) {
+  TORCH_CHECK(hidden.dim() == 2, "hidden must have shape [N, D]");
+  TORCH_CHECK(weight.dim() == 2, "weight must have shape [V, D]");
+  TORCH_CHECK(hidden.size(1) == weight.size(1), "feature dim mismatch between hidden and weight");
+  TORCH_CHECK(targets.dim() == 1 && targets.size(0) == hidden.size(0), "targets must have shape [N]");
+  TORCH_CHECK(weight.size(0) > 0 && weight.size(1) > 0, "weight must not be empty");
+  require_cuda(hidden, "hidden");
+  require_cuda(weight, "weight");
+  require_cuda(targets, "targets");
+  TORCH_CHECK(weight.device() == hidden.device() && targets.device() == hidden.device(),
+              "hidden, weight and targets must be on one device");
+  TORCH_CHECK(hidden.scalar_type() == at::kFloat || hidden.scalar_type() == at::kBFloat16,
+              "hidden must be float32 or bfloat16");
+  TORCH_CHECK(weight.scalar_type() == hidden.scalar_type(), "hidden and weight must share one dtype");
+  TORCH_CHECK(targets.scalar_type() == at::kLong || targets.scalar_type() == at::kInt, "targets must be int64 or int32");
+  TORCH_CHECK(reduction >= GRMX_REDUCE_NONE && reduction <= GRMX_REDUCE_MEAN, "reduction must be 0 (none), 1 (sum) or 2 (mean)");
+  LossArgs a;
+  a.hidden = hidden.contiguous();
+  a.weight = weight.contiguous();
+  a.targets = targets.to(at::kLong).contiguous();
+  a.N = hidden.size(0);
+  a.D = hidden.size(1);
+  a.V = weight.size(0);
+  a.dtype = a.bias_dtype = dtype_code(hidden.scalar_type(), "hidden");
+  if (bias.has_value() && bias->defined()) {
+    require_cuda(*bias, "bias");
+    TORCH_CHECK(bias->device() == hidden.device(), "bias must be on the device of hidden");
+    TORCH_CHECK(bias->dim() == 1 && bias->size(0) == a.V, "bias must have shape [V]");
+    TORCH_CHECK(bias->scalar_type() == at::kFloat || bias->scalar_type() == hidden.scalar_type(),
+                "bias must be float32 or have the dtype of hidden");
+    a.bias = bias->contiguous();
+    a.bias_dtype = dtype_code(a.bias.scalar_type(), "bias");
+  }
+  return a;
+}
+
+at::Tensor loss_workspace(const LossArgs& a, int backward) {
+  const int64_t bytes = grmx_linear_xent_workspace(a.N, a.D, a.V, a.dtype, backward);
+  TORCH_CHECK(bytes >= 0, "grm_cuda: ", grmx_last_error());
+  return at::empty({bytes}, a.hidden.options().dtype(at::kByte));
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_xent_fwd_cuda(const at::Tensor& hidden, const at::Tensor& weight,
+                                                                    const at::Tensor& targets,
+                                                                    const c10::optional<at::Tensor>& bias,
+                                                                    int64_t ignore_index, int64_t reduction) {
+  LossArgs a = check_loss_inputs(hidden, weight, targets, bias, reduction);
+  c10::cuda::CUDAGuard guard(a.hidden.device());
+  const auto f32 = a.hidden.options().dtype(at::kFloat);
+  auto loss = reduction == GRMX_REDUCE_NONE ? at::empty({a.N}, f32) : at::empty({}, f32);
+  auto stats = at::empty({2, a.N}, f32);
+  auto inv_count = at::empty({1}, f32);
+  if (a.N == 0) {      // no token: an empty list, a sum of 0, a mean of 0 / 0
+    if (reduction != GRMX_REDUCE_NONE) loss.fill_(reduction == GRMX_REDUCE_SUM ? 0.0 : std::nan(""));
+    inv_count.zero_();
+    return {loss, stats, inv_count};
+  }
+  auto ws = loss_workspace(a, 0);
+  check_status(grmx_linear_xent_fwd(a.hidden.data_ptr(), a.weight.data_ptr(), a.bias.defined() ? a.bias.data_ptr() : nullptr,
+                                    a.targets.data_ptr<int64_t>(), ignore_index, loss.data_ptr<float>(),
+                                    stats.data_ptr<float>(), inv_count.data_ptr<float>(), a.N, a.D, a.V, a.dtype,
+                                    a.bias_dtype, static_cast<int>(reduction), ws.data_ptr(), ws.numel(), current_stream()));
+  return {loss, stats, inv_count};
+}
+
+// the gradients that are asked for; the others come back empty
+std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_xent_bwd_cuda(
+    const at::Tensor& grad_loss, const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& targets,
+    const c10::optional<at::Tensor>& bias, const at::Tensor& row_stats, const at::Tensor& inv_count, int64_t ignore_index,
+    int64_t reduction, bool want_hidden, bool want_weight, bool want_bias) {
+  LossArgs a = check_loss_inputs(hidden, weight, targets, bias, reduction);
+  require_cuda(grad_loss, "grad_loss");
+  TORCH_CHECK(grad_loss.numel() == (reduction == GRMX_REDUCE_NONE ? a.N : 1), "grad_loss has the wrong number of elements");
+  TORCH_CHECK(row_stats.is_cuda() && row_stats.scalar_type() == at::kFloat && row_stats.is_contiguous() &&
+                  row_stats.numel() == 2 * a.N, "row_stats must be the float32 [2, N] of the forward call");
+  TORCH_CHECK(inv_count.is_cuda() && inv_count.scalar_type() == at::kFloat && inv_count.numel() == 1,
+              "inv_count must be the float32 [1] of the forward call");
+  TORCH_CHECK(grad_loss.device() == hidden.device() && row_stats.device() == hidden.device() &&
+                  inv_count.device() == hidden.device(), "the tensors of a backward call must be on one device");
+  TORCH_CHECK(!want_bias || a.bias.defined(), "there is no bias to differentiate");
+  c10::cuda::CUDAGuard guard(a.hidden.device());
+  auto g = grad_loss.to(at::kFloat).contiguous();
+  auto dh = want_hidden ? at::empty_like(a.hidden) : at::empty({0}, a.hidden.options());
+  auto dw = want_weight ? at::empty_like(a.weight) : at::empty({0}, a.weight.options());
+  auto db = want_bias ? at::empty_like(a.bias) : at::empty({0}, a.hidden.options());
+  if (a.N == 0) {
+    dw.zero_();
+    db.zero_();
+    return {dh, dw, db};
+  }
+  if (!want_hidden && !want_weight && !want_bias) return {dh, dw, db};
+  auto ws = loss_workspace(a, 1);
+  check_status(grmx_linear_xent_bwd(g.data_ptr<float>(), a.hidden.data_ptr(), a.weight.data_ptr(),
+                                    a.bias.defined() ? a.bias.data_ptr() : nullptr, a.targets.data_ptr<int64_t>(),
+                                    ignore_index, row_stats.data_ptr<float>(), inv_count.data_ptr<float>(),
+                                    want_hidden ? dh.data_ptr() : nullptr, want_weight ? dw.data_ptr() : nullptr,
+                                    want_bias ? db.data_ptr() : nullptr, a.N, a.D, a.V, a.dtype, a.bias_dtype,
+                                    static_cast<int>(reduction), ws.data_ptr(), ws.numel(), current_stream()));
+  return {dh, dw, db};
+}
+
+// ---- mixing rule + LayerNorm: rows [..., H] in one dtype, parameters [H] in float32 or that dtype ----
+
+struct FuseNormArgs {
+  at::Tensor online, update, gate, scale, weight, bias;
+  int64_t rows, H;
+  int dtype, param_dtype;
+};
+
+FuseNormArgs check_fuse_norm_inputs(const at::Tensor& online, const at::Tensor& update, const c10::optional<at::Tensor>& gate,
+                                    const c10::optional<at::Tensor>& scale, const c10::optional<at::Tensor>& ln_weight,
+                                    const c10::optional<at::Tensor>& ln_bias) {
+  TORCH_CHECK(online.dim() >= 1 && online.size(-1) > 0, "online must have shape [..., H]");
+  require_cuda(online, "online");
+  TORCH_CHECK(online.scalar_type() == at::kFloat || online.scalar_type() == at::kBFloat16,
+              "online must be float32 or bfloat16");
+  FuseNormArgs a;
+  a.H = online.size(-1);
+  a.rows = online.numel() / a.H;
+  a.dtype = dtype_code(online.scalar_type(), "online");
+  a.param_dtype = GRMX_F32;
+  auto row_tensor = [&](const at::Tensor& t, const char* name) {
+    require_cuda(t, name);
+    TORCH_CHECK(t.sizes() == online.sizes(), name, " must have the shape of online");
+    TORCH_CHECK(t.scalar_type() == online.scalar_type(), name, " must have the dtype of online");
+    TORCH_CHECK(t.device() == online.device(), name, " must be on the device of online");
+    return t.contiguous();
+  };
+  bool first = true;
+  auto param = [&](const c10::optional<at::Tensor>& t, const char* name) {
+    if (!t.has_value() || !t->defined()) return at::Tensor();
+    require_cuda(*t, name);
+    TORCH_CHECK(t->dim() == 1 && t->size(0) == a.H, name, " must have shape [H]");
+    TORCH_CHECK(t->device() == online.device(), name, " must be on the device of online");
+    TORCH_CHECK(t->scalar_type() == at::kFloat || t->scalar_type() == online.scalar_type(),
+                name, " must be float32 or have the dtype of online");
+    const int code = dtype_code(t->scalar_type(), name);
+    TORCH_CHECK(first || code == a.param_dtype, "scale, ln_weight and ln_bias must share one dtype");
+    first = false;
+    a.param_dtype = code;
+    return t->contiguous();
+  };
+  a.online = online.contiguous();
+  a.update = row_tensor(update, "update");
+  if (gate.has_value() && gate->defined()) a.gate = row_tensor(*gate, "gate");
+  a.scale = param(scale, "scale");
+  a.weight = param(ln_weight, "ln_weight");
+  a.bias = param(ln_bias, "ln_bias");
+  return a;
+}
+
+void* ptr_or_null(const at::Tensor& t) { return t.defined() && t.numel() > 0 ? t.data_ptr() : nullptr; }
+
+// out, sum (empty unless asked for), row statistics [rows, 2] (empty unless asked for)
+std::tuple<at::Tensor, at::Tensor, at::Tensor> fuse_norm_fwd_cuda(
+    const at::Tensor& online, const at::Tensor& update, const c10::optional<at::Tensor>& gate,
+    const c10::optional<at::Tensor>& scale, const c10::optional<at::Tensor>& ln_weight,
+    const c10::optional<at::Tensor>& ln_bias, double eps, bool want_sum, bool want_stats) {
+  FuseNormArgs a = check_fuse_norm_inputs(online, update, gate, scale, ln_weight, ln_bias);
+  c10::cuda::CUDAGuard guard(a.online.device());
+  auto out = at::empty_like(a.online);
+  auto sum = want_sum ? at::empty_like(a.online) : at::empty({0}, a.online.options());
+  const auto f32 = a.online.options().dtype(at::kFloat);
+  auto stats = want_stats ? at::empty({a.rows, 2}, f32) : at::empty({0}, f32);
+  check_status(grmx_fuse_norm_fwd(a.online.data_ptr(), a.update.data_ptr(), ptr_or_null(a.gate), ptr_or_null(a.scale),
+                                  ptr_or_null(a.weight), ptr_or_null(a.bias), static_cast<float>(eps), out.data_ptr(),
+                                  ptr_or_null(sum), static_cast<float*>(ptr_or_null(stats)), a.rows, a.H, a.dtype,
+                                  a.param_dtype, current_stream()));
+  return {out, sum, stats};
+}
+
+// gradients of online, update, gate, scale, ln_weight, ln_bias; those that are not asked for come back empty
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> fuse_norm_bwd_cuda(
+    const c10::optional<at::Tensor>& grad_out, const c10::optional<at::Tensor>& grad_sum, const at::Tensor& online,
+    const at::Tensor& update, const c10::optional<at::Tensor>& gate, const c10::optional<at::Tensor>& scale,
+    const c10::optional<at::Tensor>& ln_weight, const c10::optional<at::Tensor>& ln_bias, const at::Tensor& row_stats,
+    c10::List<bool> want) {
+  TORCH_CHECK(want.size() == 6, "want must name six gradients");
+  FuseNormArgs a = check_fuse_norm_inputs(online, update, gate, scale, ln_weight, ln_bias);
+  TORCH_CHECK(row_stats.is_cuda() && row_stats.device() == a.online.device() && row_stats.scalar_type() == at::kFloat &&
+                  row_stats.is_contiguous() && row_stats.numel() == 2 * a.rows,
+              "row_stats must be the float32 [rows, 2] of the forward call");
+  TORCH_CHECK(!want[2] || a.gate.defined(), "there is no gate to differentiate");
+  TORCH_CHECK(!want[3] || a.scale.defined(), "there is no scale to differentiate");
+  TORCH_CHECK((!want[4] || a.weight.defined()) && (!want[5] || a.bias.defined()), "there is no ln_weight or ln_bias to differentiate");
+  c10::cuda::CUDAGuard guard(a.online.device());
+  auto grad = [&](const c10::optional<at::Tensor>& t, const char* name) {
+    if (!t.has_value() || !t->defined()) return at::Tensor();
+    require_cuda(*t, name);
+    TORCH_CHECK(t->numel() == a.online.numel() && t->device() == a.online.device(), name, " does not fit online");
+    return t->to(a.online.scalar_type()).contiguous();
+  };
+  at::Tensor dy = grad(grad_out, "grad_out"), dsum = grad(grad_sum, "grad_sum");
+  TORCH_CHECK(dy.defined() || dsum.defined(), "neither output has a gradient");
+  auto like = [&](const at::Tensor& t, bool wanted) {
+    return wanted ? at::empty_like(t) : at::empty({0}, a.online.options());
+  };
+  auto d_online = like(a.online, want[0]), d_update = like(a.update, want[1]), d_gate = like(a.gate, want[2]);
+  auto d_scale = like(a.scale, want[3]), d_weight = like(a.weight, want[4]), d_bias = like(a.bias, want[5]);
+  const int64_t bytes = grmx_fuse_norm_workspace(a.rows, a.H);
+  TORCH_CHECK(bytes >= 0, "grm_cuda: ", grmx_last_error());
+  const bool columns = want[3] || want[4] || want[5];
+  auto ws = at::empty({columns ? bytes : 0}, a.online.options().dtype(at::kByte));
+  check_status(grmx_fuse_norm_bwd(ptr_or_null(dy), ptr_or_null(dsum), a.online.data_ptr(), a.update.data_ptr(),
+                                  ptr_or_null(a.gate), ptr_or_null(a.scale), ptr_or_null(a.weight),
+                                  row_stats.data_ptr<float>(), ptr_or_null(d_online), ptr_or_null(d_update),
+                                  ptr_or_null(d_gate), ptr_or_null(d_scale), ptr_or_null(d_weight), ptr_or_null(d_bias),
+                                  a.rows, a.H, a.dtype, a.param_dtype, ptr_or_null(ws), ws.numel(), current_stream()));
+  return {d_online, d_update, d_gate, d_scale, d_weight, d_bias};
+}
+
 }  // namespace
 
 TORCH_LIBRARY(grm_cuda, m) {
@@ -577,6 +798,10 @@ TORCH_LIBRARY(grmx, m) {
   m.def("project_normalize(Tensor x, Tensor weights, Tensor? bias, float eps) -> (Tensor a, Tensor b)");
   m.def("archive_push(Tensor memory, Tensor(a!) archive, Tensor(b!)? shadow, int slot) -> ()");
   m.def("add_layer_norm(Tensor a, Tensor b, Tensor? ln_weight, Tensor? ln_bias, float ln_eps) -> Tensor");
+  m.def("linear_xent_fwd(Tensor hidden, Tensor weight, Tensor targets, Tensor? bias, int ignore_index, int reduction) -> (Tensor loss, Tensor row_stats, Tensor inv_count)");
+  m.def("linear_xent_bwd(Tensor grad_loss, Tensor hidden, Tensor weight, Tensor targets, Tensor? bias, Tensor row_stats, Tensor inv_count, int ignore_index, int reduction, bool want_hidden, bool want_weight, bool want_bias) -> (Tensor grad_hidden, Tensor grad_weight, Tensor grad_bias)");
+  m.def("fuse_norm_fwd(Tensor online, Tensor update, Tensor? gate, Tensor? scale, Tensor? ln_weight, Tensor? ln_bias, float eps, bool want_sum, bool want_stats) -> (Tensor out, Tensor sum, Tensor row_stats)");
+  m.def("fuse_norm_bwd(Tensor? grad_out, Tensor? grad_sum, Tensor online, Tensor update, Tensor? gate, Tensor? scale, Tensor? ln_weight, Tensor? ln_bias, Tensor row_stats, bool[] want) -> (Tensor grad_online, Tensor grad_update, Tensor grad_gate, Tensor grad_scale, Tensor grad_weight, Tensor grad_bias)");
   m.def("select_fuse(Tensor states, Tensor indices, Tensor gates, Tensor? online, Tensor? ln_weight, Tensor? ln_bias, float ln_eps, int mode) -> Tensor");
 }
 
@@ -586,6 +811,10 @@ TORCH_LIBRARY_IMPL(grmx, CUDA, m) {
   m.impl("topk_select", topk_select_cuda);
   m.impl("retrieve_fuse", retrieve_fuse_cuda);
   m.impl("retrieve_fuse_tc", retrieve_fuse_tc_cuda);
+  m.impl("linear_xent_fwd", linear_xent_fwd_cuda);
+  m.impl("linear_xent_bwd", linear_xent_bwd_cuda);
+  m.impl("fuse_norm_fwd", fuse_norm_fwd_cuda);
+  m.impl("fuse_norm_bwd", fuse_norm_bwd_cuda);
   m.impl("select_fuse", select_fuse_cuda);
   m.impl("add_layer_norm", add_layer_norm_cuda);
   m.impl("archive_push", archive_push_cuda);

@@ -47,6 +47,7 @@ _POLICY_ENV = {
 _ERROR_BITS = {
     1: "an index outside the archive reached a gather or retrieval kernel (the row was zero-filled)",
     2: "a bounded wait inside a tensor-core kernel gave up (outputs of that call are incomplete)",
+    4: "a target outside the vocabulary reached the loss (the token was ignored)",
 }
 
 

@@ -1,0 +1,74 @@
+"""Softmax cross entropy of the vocabulary projection, with its gradient, without keeping the scores.
+
+The language-model wrapper of the reference projects its last hidden states onto the vocabulary
+(grm/utils/train.py:223) and hands the ``[tokens, vocabulary]`` scores to the cross entropy.  Here
+projection and loss are one operator: the scores exist tile by tile on the tensor cores, forward and (a second
+time) backward.  The kernels are ``grmx_linear_xent_fwd`` / ``grmx_linear_xent_bwd`` of the C ABI.
+CUDA tensors only.
+"""
+
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+from torch import Tensor
+from torch.autograd.function import once_differentiable
+
+from . import cuda_ops
+
+_REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
+
+
+class LinearCrossEntropyFn(torch.autograd.Function):
+    """``hidden [N, D], weight [V, D], targets [N], bias [V]?`` -> loss ``[N]`` or scalar, float32."""
+
+    @staticmethod
+    def forward(ctx, hidden: Tensor, weight: Tensor, targets: Tensor, bias: Optional[Tensor], ignore_index: int,
+                reduction: int):
+        loss, row_stats, inv_count = torch.ops.grmx.linear_xent_fwd(hidden, weight, targets, bias, ignore_index, reduction)
+        ctx.save_for_backward(hidden, weight, targets, bias, row_stats, inv_count)
+        ctx.ignore_index, ctx.reduction = ignore_index, reduction
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_loss: Tensor):
+        hidden, weight, targets, bias, row_stats, inv_count = ctx.saved_tensors
+        want = (ctx.needs_input_grad[0], ctx.needs_input_grad[1], ctx.needs_input_grad[3])
+        grads = torch.ops.grmx.linear_xent_bwd(grad_loss, hidden, weight, targets, bias, row_stats, inv_count,
+                                               ctx.ignore_index, ctx.reduction, *want)
+        d_hidden, d_weight, d_bias = (grad if wanted else None for grad, wanted in zip(grads, want))
+        return d_hidden, d_weight, None, d_bias, None, None
+
+
+def linear_cross_entropy(hidden: Tensor, weight: Tensor, targets: Tensor, bias: Optional[Tensor] = None, *,
+                         ignore_index: int = -100, reduction: str = "mean") -> Tensor:
+    """``cross_entropy(hidden @ weight.T + bias, targets)`` in float32, for ``hidden [..., D]`` and ``targets [...]``.
+
+    ``hidden`` and ``weight [V, D]`` share one type, bfloat16 or float32; ``bias [V]`` has that type or is
+    float32; gradients come in the types of what they belong to.  ``reduction`` is "none" (``[...]``), "sum" or
+    "mean" (over the tokens that count; NaN if none does).  Tokens with ``target == ignore_index`` have loss 0 and
+    a zero gradient.  Any other target outside the vocabulary is ignored too and reported by
+    ``cuda_ops.check_device_errors``.  A word whose bias is ``-inf`` is masked: it has probability 0.
+    The hidden states of ignored tokens must be finite (they are multiplied by a zero gradient).
+    """
+    cuda_ops._require_extension("linear_cross_entropy")
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"reduction must be one of {sorted(_REDUCTIONS)}, got {reduction!r}")
+    if hidden.device.type != "cuda":
+        raise RuntimeError(f"linear_cross_entropy: tensors must be on a CUDA device, got {hidden.device}; this engine has no "
+                           "CPU path.")
+    if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1]:
+        raise ValueError(f"hidden [..., D] and weight [V, D] do not fit: {tuple(hidden.shape)}, {tuple(weight.shape)}")
+    if targets.shape != hidden.shape[:-1]:
+        raise ValueError(f"targets must have the shape {tuple(hidden.shape[:-1])}, got {tuple(targets.shape)}")
+    rows, flat = hidden.reshape(-1, hidden.shape[-1]), targets.reshape(-1)
+    code = _REDUCTIONS[reduction]
+    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
+        loss = LinearCrossEntropyFn.apply(rows, weight, flat, bias, int(ignore_index), code)
+    else:
+        loss = torch.ops.grmx.linear_xent_fwd(rows, weight, flat, bias, int(ignore_index), code)[0]
+    if cuda_ops._checking_each_call() and not torch.cuda.is_current_stream_capturing():
+        cuda_ops.check_device_errors()
+    return loss.reshape(targets.shape) if reduction == "none" else loss

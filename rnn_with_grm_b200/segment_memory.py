@@ -36,6 +36,7 @@ import torch.nn.functional as F
 from torch import Tensor
 
 from . import cuda_ops
+from .loss import linear_cross_entropy
 
 FUSE_RETRIEVED, FUSE_CONTRIB, FUSE_RESIDUAL_LN = 0, 1, 2
 
@@ -750,8 +751,8 @@ class StackedSegmentMemoryRunner:
             params.append(cached[1])
         return torch.ops.grmx.add_layer_norm(h, out, params[0], params[1], 1e-5)
 
-    @torch.no_grad()
-    def forward(self, x: Tensor, reset_memory: bool = True):
+    def _body(self, x: Tensor, reset_memory: bool) -> Tuple[Tensor, Tensor]:
+        """Everything up to the stack's own output projection: ``(y [B, T, hidden], final memories)``."""
         p, pre = self.params, self.prefix
         B, T = x.shape[0], x.shape[1]
         lengths = {layer.segment_length for layer in self.layers}
@@ -777,10 +778,29 @@ class StackedSegmentMemoryRunner:
         if segment_major:
             h = h.transpose(0, 1).reshape(B, T, h.shape[-1])
         y = F.linear(h, p[f"{pre}output_proj.weight"], p.get(f"{pre}output_proj.bias"))
-        if self.language_model and self.vocabulary_projection:
-            y = F.linear(y, p["output_layer.weight"], p.get("output_layer.bias"))
-        _check_errors_if_asked()
         return y, torch.stack(finals, dim=0)
+
+    @torch.no_grad()
+    def forward(self, x: Tensor, reset_memory: bool = True):
+        y, finals = self._body(x, reset_memory)
+        if self.language_model and self.vocabulary_projection:
+            y = F.linear(y, self.params["output_layer.weight"], self.params.get("output_layer.bias"))
+        _check_errors_if_asked()
+        return y, finals
+
+    @torch.no_grad()
+    def loss(self, ids: Tensor, targets: Tensor, *, reset_memory: bool = True, ignore_index: int = -100,
+             reduction: str = "mean") -> Tensor:
+        """Cross entropy of the language model's next-word scores against ``targets [B, T]`` (float32), as
+        ``cross_entropy(forward(ids), targets)`` would give it, without the ``[B, T, vocabulary]`` scores: the
+        vocabulary projection runs inside the loss (``loss.linear_cross_entropy``)."""
+        if not self.language_model:
+            raise ValueError("loss() needs the language-model wrapper (language_model=True)")
+        if targets.shape != ids.shape:
+            raise ValueError(f"targets must have the shape {tuple(ids.shape)} of ids, got {tuple(targets.shape)}")
+        y, _ = self._body(ids, reset_memory)
+        return linear_cross_entropy(y, self.params["output_layer.weight"], targets, self.params.get("output_layer.bias"),
+                                    ignore_index=ignore_index, reduction=reduction)
 
 
 class GraphedForward:
