@@ -307,8 +307,15 @@ int launch_pair(const Maps& maps, const Params& p, const char* what, cudaStream_
   const int64_t units = static_cast<int64_t>(p.m_tiles) * p.n_tiles * p.splits;
   const int pairs = pairs_on_device();
   const unsigned grid = 2u * static_cast<unsigned>(units < pairs ? units : pairs);
-  kernel<<<grid, kThreads, kSmemAlloc, s>>>(maps, p, device_error_word_ptr());
+  kernel<<<grid, threads_of(EPI, SEG), kSmemAlloc, s>>>(maps, p, device_error_word_ptr());
   return check_launch(what);
+}
+
+// the products whose epilogue works on scores
+template <int EPI>
+int launch_scores(const Maps& maps, const Params& p, int dtype, const char* what, cudaStream_t s) {
+  if (dtype == GRMX_F32) return launch_pair<EPI, false, false, true>(maps, p, what, s);
+  return launch_pair<EPI, false, false, false>(maps, p, what, s);
 }
 
 // A K-major operand tile is one box of 64 k x 128 rows; an MN-major one is two boxes of 64 columns x 64 k.
@@ -385,7 +392,7 @@ struct ForwardPlan {
 
 ForwardPlan plan_forward(int64_t N, int64_t D, int64_t V, int dtype) {
   ForwardPlan f;
-  f.parts = static_cast<int>(ceil_div(V, kTileN)) * (dtype == GRMX_F32 ? 2 : 1);
+  f.parts = static_cast<int>(ceil_div(V, kTileN)) * parts_of(kEpiLse, dtype == GRMX_F32);
   f.join_blocks = ceil_div(N, kJoinRows);
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
@@ -480,8 +487,7 @@ extern "C" int grmx_linear_xent_fwd(const void* hidden, const void* weight, cons
   p.partials = reinterpret_cast<float2*>(ws + f.off_part);
   p.target_score = reinterpret_cast<float*>(ws + f.off_target);
   p.ticket = reinterpret_cast<uint32_t*>(ws + f.off_ticket);
-  GRMX_TRY(dtype == GRMX_F32 ? (launch_pair<kEpiLse, false, false, true>(maps, p, "loss scores", s))
-                             : (launch_pair<kEpiLse, false, false, false>(maps, p, "loss scores", s)));
+  GRMX_TRY(launch_scores<kEpiLse>(maps, p, dtype, "loss scores", s));
   loss_join_kernel<<<static_cast<unsigned>(f.join_blocks), kJoinRows * kJoinSlices, 0, s>>>(
       p.partials, p.target_score, targets, ignore_index, V, N, f.parts, reduction, row_stats, row_stats + N, loss, inv_count,
       reinterpret_cast<double*>(ws + f.off_loss), reinterpret_cast<int*>(ws + f.off_count), p.ticket, device_error_word_ptr());
@@ -540,12 +546,15 @@ extern "C" int grmx_linear_xent_bwd(const float* grad_loss, const void* hidden, 
     const Operand w_piece{static_cast<const uint8_t*>(w.ptr) + v0 * w.ld * 2, w.ld, w.plane_stride, w.planes};
     {
       Maps maps;
-      if (!operand_map(&maps.a, x, N, D, false) || !operand_map(&maps.b, w_piece, words, D, false) ||
-          !make_matrix_map(&maps.c, d.ptr, false, planes, N, width, d.ld, d.plane_stride, 64, 128)) {
+      if (!operand_map(&maps.a, x, N, D, false) || !operand_map(&maps.b, w_piece, words, D, false)) {
         return fail(GRMX_ERR_LAUNCH, "%s: cuTensorMapEncodeTiled failed", who);
       }
+      maps.c = maps.a;
       Params p;
       memset(&p, 0, sizeof(p));
+      p.d_out = reinterpret_cast<__nv_bfloat16*>(ws + b.off_d);
+      p.d_ld = d.ld;
+      p.d_plane_stride = d.plane_stride;
       p.m_tiles = static_cast<int>(ceil_div(N, kTileM));
       p.n_tiles = static_cast<int>(width / kTileN);
       p.splits = 1;
@@ -562,8 +571,7 @@ extern "C" int grmx_linear_xent_bwd(const float* grad_loss, const void* hidden, 
       p.row_sum = row_stats + N;
       p.grad = reduction == GRMX_REDUCE_NONE ? grad_loss : nullptr;
       p.bias_partials = grad_bias != nullptr ? part_b : nullptr;
-      GRMX_TRY(f32 ? (launch_pair<kEpiGrad, false, false, true>(maps, p, "loss score gradient", s))
-                   : (launch_pair<kEpiGrad, false, false, false>(maps, p, "loss score gradient", s)));
+      GRMX_TRY(launch_scores<kEpiGrad>(maps, p, dtype, "loss score gradient", s));
     }
     if (grad_bias != nullptr) {
       const int64_t blocks = ceil_div(N, kTileM) * 8;

@@ -5,8 +5,8 @@
 // Each CTA of a pair holds 128 rows of A and 128 of the 256 columns of B in shared memory (32 KiB per
 // 64-wide k block), and its own 128 rows of the result in TMEM: a pair reads (256 + 256) * 64 values per
 // 2 * 256 * 256 * 64 FLOP, half of what a single CTA with a 128 x 256 tile would ask of L2 for its share,
-// which is what decides whether the tensor cores are fed.  Persistent pairs; warp 8 loads (TMA ring of
-// kStages blocks), warp 9 of the first CTA issues for both, warps 0-7 are the epilogue.  Two accumulators
+// which is what decides whether the tensor cores are fed.  Persistent pairs; one warp loads (TMA ring of
+// kStages blocks), one warp of the first CTA issues for both, the others are the epilogue in groups of four.  Two accumulators
 // of 256 columns: the epilogue of a tile runs under the products of the next one.
 //
 // Operands are bf16 matrices [planes][rows][cols] read through tensor maps; either may be K-major (k is the
@@ -30,27 +30,36 @@ constexpr int kTileM = 256;              // rows per pair
 constexpr int kTileN = 256;              // columns per pair
 constexpr int kHalf = 128;               // rows of A, columns of B and rows of the result per CTA
 constexpr int kBlockK = 64;
-constexpr int kStages = 5;
 constexpr int kOperandBytes = kHalf * kBlockK * 2;       // 16 KiB
-constexpr int kStageBytes = 2 * kOperandBytes;
-constexpr int kThreads = 320;
-constexpr int kLoaderWarp = 8;
-constexpr int kIssuerWarp = 9;
 constexpr int kGroupThreads = 128;       // an epilogue group: one warp per TMEM lane quadrant
-constexpr int kStoreBytes = 16384;       // staging buffer: 128 rows x 128 bytes
-constexpr int kOffStore = kStages * kStageBytes;         // [group][2]
-constexpr int kOffBias = kOffStore + 4 * kStoreBytes;    // float[2][256]
-constexpr int kOffBars = kOffBias + 2 * kTileN * 4;
+constexpr int kStoreBytes = 16384;       // staging buffer of a TMA store: 128 rows x 128 bytes
+constexpr int kBiasBytes = 2048;         // float[512] among the epilogue groups
+constexpr int kSmemAlloc = 232448;
+
+constexpr int kStages = 5;
+constexpr int kStageBytes = 2 * kOperandBytes;           // [A | B]
+constexpr int kOffStore = kStages * kStageBytes;         // staging of the epilogue groups
+constexpr int kOffBias = kOffStore + 4 * kStoreBytes;
+constexpr int kOffBars = kOffBias + kBiasBytes;
 constexpr int kNumBars = 2 * kStages + 4;
 constexpr int kOffMisc = kOffBars + kNumBars * 8;
 constexpr int kSmemTotal = kOffMisc + 32;
-constexpr int kSmemAlloc = 232448;
 static_assert(kSmemTotal <= kSmemAlloc, "shared memory plan exceeds 227 KiB");
 static_assert(kOffBars % 8 == 0, "barriers are 8-byte aligned");
 // k blocks between two drains of the accumulator in full precision: 32 blocks are 128 accumulations
 constexpr int kSegmentSteps = 32;
 
 enum Epilogue { kEpiLse = 0, kEpiGrad = 1, kEpiStore = 2 };
+
+// Epilogue groups of four warps: four where the epilogue has an exponential per score (two on each accumulator, 128
+// columns each; with two groups the epilogue of a tile took longer than its products, 414 against 385 us for 16384 x
+// 32768 scores of 512 terms, and with three 737 against 594 us where it also writes the gradient), two for plain
+// results (one per accumulator).  In full precision four, each on 64 columns of every accumulator, because the drained
+// accumulator has to fit in a thread's registers (with two groups and 128 columns it spilled).
+__host__ __device__ constexpr int groups_of(int epilogue, bool seg) { return !seg && epilogue == kEpiStore ? 2 : 4; }
+__host__ __device__ constexpr int threads_of(int epilogue, bool seg) { return groups_of(epilogue, seg) * kGroupThreads + 64; }
+// column parts of a tile that different groups work on
+__host__ __device__ constexpr int parts_of(int epilogue, bool seg) { return seg ? 4 : groups_of(epilogue, seg) / 2; }
 
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -74,7 +83,9 @@ struct Params {
   const float* row_max;        // [rows], base 2
   const float* row_sum;
   const float* grad;           // [rows], or NULL: 1 (a factor that all rows share is applied to the results)
-  float* bias_partials;        // [row blocks of 128][n_tiles * 256] or NULL
+  float* bias_partials;        // [row blocks of 32][n_tiles * 256] or NULL
+  __nv_bfloat16* d_out;        // [planes][rows][d_ld]
+  int64_t d_ld, d_plane_stride;
   // kEpiStore
   int store_f32;               // the store map is fp32 (32-column boxes) instead of bf16 (64)
   int store_add;               // add to what is there (fp32 only)
@@ -100,26 +111,15 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// Arrival on a barrier of either CTA.  What it hands over is an accumulator, which the tcgen05 fences order; a release at
+// cluster scope would also wait for this thread's stores to memory (a fence per arrival).
 __device__ __forceinline__ void arrive_cluster(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
-}
-__device__ __forceinline__ uint32_t try_wait_cluster(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t"
-      ".reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t"
-      "}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok;
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 // bounded wait; giving up raises the abort flag of both CTAs
 __device__ __forceinline__ bool wait_pair(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
   for (uint32_t it = 0; it < kWaitLimit; ++it) {
-    if (try_wait_cluster(bar, parity)) return true;
+    if (mbar_try_wait(bar, parity)) return true;
     if ((it & 63u) == 63u && *abort_flag) return false;
   }
   *abort_flag = 1;
@@ -201,24 +201,114 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
-// unit of work -> (row tile, column tile, split)
-template <int EPI>
-__device__ __forceinline__ void unit_to_tile(const Params& p, int u, int& m, int& n, int& s) {
-  if (EPI == kEpiStore) {
-    // column tiles of a row tile next to each other: they read the same A
-    n = u % p.n_tiles;
-    m = (u / p.n_tiles) % p.m_tiles;
-    s = u / (p.n_tiles * p.m_tiles);
-  } else {
-    // bands of eight row tiles, column by column: the tiles that run at one time share rows and columns in L2
-    const int per_band = 8 * p.n_tiles;
-    const int band = u / per_band, r = u % per_band;
-    const int height = min(8, p.m_tiles - 8 * band);
-    m = 8 * band + r % height;
-    n = r / height;
-    s = 0;
+// two fp32 operations per instruction
+__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// y = score * log2 e + bias * log2 e for 32 columns (bias already scaled, 16-byte aligned)
+__device__ __forceinline__ void scores_base2(float (&y)[32], const float* bias) {
+  const uint64_t k = pack2(kLog2e, kLog2e);
+#pragma unroll
+  for (int j = 0; j < 32; j += 4) {
+    const float4 b = *reinterpret_cast<const float4*>(bias + j);
+    unpack2(fma2(pack2(y[j], y[j + 1]), k, pack2(b.x, b.y)), y[j], y[j + 1]);
+    unpack2(fma2(pack2(y[j + 2], y[j + 3]), k, pack2(b.z, b.w)), y[j + 2], y[j + 3]);
   }
 }
+
+// 32 rows x 32 bf16 that a warp stages for itself: 64 bytes per row, 16-byte pieces swizzled by the row so that neither
+// the rows' writes nor the reads below collide.
+__device__ __forceinline__ uint8_t* box_piece(uint8_t* box, int row, int piece) {
+  return box + row * 64 + ((piece ^ ((row >> 1) & 3)) << 4);
+}
+// The box to memory, eight rows at a time, its columns added up in fp32 on the way (a lane moves four rows of eight
+// columns, the eight lanes of a column then share out the sums).  `out` is the box's first value; rows at and beyond
+// `rows` are not stored.  Returns the sums of columns box_column(lane) and the next, in both lanes of a pair 4 apart.
+// (A TMA store needs the whole group's barriers and a wait of 0.8 us until its buffer is free again.)
+__device__ __forceinline__ int box_column(int lane) { return (lane & 3) * 8 + ((lane >> 4) & 1) * 4 + ((lane >> 3) & 1) * 2; }
+template <bool SUMS>
+__device__ __forceinline__ float2 box_out(uint8_t* box, __nv_bfloat16* out, int64_t ld, int rows, int lane) {
+  const int q = lane & 3, sub = lane >> 2;
+  uint64_t acc[4] = {0ull, 0ull, 0ull, 0ull};
+  __nv_bfloat16* dst = out + sub * ld + q * 8;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const uint4 v = *reinterpret_cast<const uint4*>(box_piece(box, 8 * r + sub, q));
+    if (8 * r + sub < rows) *reinterpret_cast<uint4*>(dst) = v;
+    dst += 8 * ld;
+    if (SUMS) {
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] = add2(acc[e], pack2(__uint_as_float(w[e] << 16), __uint_as_float(w[e] & 0xffff0000u)));
+    }
+  }
+  float2 sums = make_float2(0.0f, 0.0f);
+  if (SUMS) {
+    // lanes 16 apart, then 8 apart, give away the half they do not return; lanes 4 apart return the same
+    const bool upper = (lane & 16) != 0, odd = (lane & 8) != 0;
+    uint64_t half[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const uint64_t keep = upper ? acc[2 + e] : acc[e], give = upper ? acc[e] : acc[2 + e];
+      half[e] = add2(keep, __shfl_xor_sync(0xffffffffu, give, 16));
+    }
+    uint64_t one = odd ? half[1] : half[0];
+    const uint64_t give = odd ? half[0] : half[1];
+    one = add2(one, __shfl_xor_sync(0xffffffffu, give, 8));
+    one = add2(one, __shfl_xor_sync(0xffffffffu, one, 4));
+    unpack2(one, sums.x, sums.y);
+  }
+  return sums;
+}
+
+// The units of work of one pair and what each of them is.
+template <int EPI>
+struct Units {
+  int begin, end, step;
+  __device__ __forceinline__ Units(const Params& p) {
+    const int total = p.m_tiles * p.n_tiles * p.splits, pairs = gridDim.x >> 1, pair = blockIdx.x >> 1;
+    begin = pair;
+    end = total;
+    step = pairs;
+  }
+  // row tile, column tile, split
+  __device__ __forceinline__ void tile(const Params& p, int u, int& m, int& n, int& s) const {
+    s = 0;
+    if (EPI == kEpiStore) {
+      // column tiles of a row tile next to each other: they read the same A
+      n = u % p.n_tiles;
+      m = (u / p.n_tiles) % p.m_tiles;
+      s = u / (p.n_tiles * p.m_tiles);
+    } else {
+      // bands of eight row tiles, column by column: the tiles that run at one time share rows and columns in L2
+      const int per_band = 8 * p.n_tiles;
+      const int band = u / per_band, r = u % per_band;
+      const int height = min(8, p.m_tiles - 8 * band);
+      m = 8 * band + r % height;
+      n = r / height;
+    }
+  }
+};
 
 // Sums over the 32 lanes of a warp of 32 values each; lane j returns the sum of v[j].
 __device__ __forceinline__ float transpose_sum(float (&v)[32], int lane) {
@@ -235,11 +325,74 @@ __device__ __forceinline__ float transpose_sum(float (&v)[32], int lane) {
   return v[0];
 }
 
+// biases of `count` words from word v, base 2, into shared memory; words beyond the vocabulary get -inf
+__device__ __forceinline__ void load_bias(const Params& p, float* dst, int64_t v, int count, int thread, int threads) {
+  for (int j = thread; j < count; j += threads) {
+    float b = -INFINITY;
+    if (v + j < p.vocab) {
+      b = 0.0f;
+      if (p.bias != nullptr) {
+        b = p.bias_dtype == GRMX_F32 ? __ldg(static_cast<const float*>(p.bias) + v + j)
+                                     : __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(p.bias) + v + j));
+      }
+    }
+    dst[j] = b * kLog2e;
+  }
+}
+
+// d = g * (2^(y - top) / sum - [target]) = coef * 2^(y - top) - [target] g; a row that does not count is all zero
+struct RowTerms {
+  int64_t target;              // word of the target relative to the first column, or -1
+  float top, coef, g;
+  bool counts;
+};
+__device__ __forceinline__ RowTerms row_terms(const Params& p, int64_t row, int64_t first_word) {
+  RowTerms r{-1, 0.0f, 0.0f, 0.0f, false};
+  if (row < p.rows) {
+    const int64_t t = __ldg(p.targets + row);
+    if (t != p.ignore_index && t >= 0 && t < p.vocab) {
+      if (t >= first_word) r.target = t - first_word;
+      r.g = p.grad != nullptr ? __ldg(p.grad + row) : 1.0f;
+      r.top = __ldg(p.row_max + row);
+      r.coef = r.g / __ldg(p.row_sum + row);
+      r.counts = r.coef != 0.0f || r.g != 0.0f;
+    }
+  }
+  return r;
+}
+// 32 scores to their gradients; `first` is the columns' place relative to the one r.target counts from
+__device__ __forceinline__ void score_gradient(float (&y)[32], const float* bias, const RowTerms& r, int first) {
+  scores_base2(y, bias);
+  const uint64_t shift = pack2(-r.top, -r.top), factor = pack2(r.coef, r.coef);
+#pragma unroll
+  for (int j = 0; j < 32; j += 2) {
+    float lo, hi;
+    unpack2(add2(pack2(y[j], y[j + 1]), shift), lo, hi);
+    unpack2(mul2(pack2(exp2_fast(lo), exp2_fast(hi)), factor), y[j], y[j + 1]);
+  }
+  if (!__all_sync(0xffffffffu, r.counts)) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) y[j] = r.counts ? y[j] : 0.0f;
+  }
+  const bool hit = r.target >= first && r.target < first + 32;
+  if (__any_sync(0xffffffffu, hit)) {
+    const int at = hit ? static_cast<int>(r.target) - first : -1;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      if (at == j) y[j] -= r.g;
+    }
+  }
+}
+
 // SEG: full precision (six plane products, accumulator drained into registers; both epilogue groups work on
-// every tile, 128 columns each).  Otherwise the groups take alternate tiles, one accumulator each.
+// every tile).  Otherwise half of the groups work on each accumulator, so on every other tile.
 template <int EPI, bool A_MN, bool B_MN, bool SEG>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(EPI, SEG), 1)
 pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p, uint32_t* error_word) {
+  constexpr int kGroups = groups_of(EPI, SEG);
+  constexpr int kParts = parts_of(EPI, SEG);
+  constexpr int kLoaderWarp = 4 * kGroups;
+  constexpr int kIssuerWarp = kLoaderWarp + 1;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kOffBars);
@@ -267,7 +420,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bar_acc_ready[i], 1);
-      mbar_init(&bar_acc_free[i], SEG ? 16 : 8);
+      mbar_init(&bar_acc_free[i], 8 * kParts);
     }
     *s_abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -285,9 +438,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
   tc_fence_after();
   const uint32_t tmem_base = *s_tmem;
 
-  const int units = p.m_tiles * p.n_tiles * p.splits;
-  const int n_pairs = gridDim.x >> 1;
-  const int pair_id = blockIdx.x >> 1;
+  const Units<EPI> units(p);
   auto split_range = [&](int s, int& k0, int& k1) {
     k0 = s * p.blocks_per_split;
     k1 = min(p.k_blocks, k0 + p.blocks_per_split);
@@ -301,32 +452,32 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
     // plane products, smallest first: (low, high) (high, low) (mid, mid) (mid, high) (high, mid) (high, high)
     constexpr uint32_t kPlaneA = 2u | (0u << 2) | (1u << 4) | (1u << 6) | (0u << 8) | (0u << 10);
     constexpr uint32_t kPlaneB = 0u | (2u << 2) | (1u << 4) | (0u << 6) | (1u << 8) | (0u << 10);
-    for (int u = pair_id; u < units && ok; u += n_pairs) {
+    for (int u = units.begin; u < units.end && ok; u += units.step) {
       int m, n, s, k0, k1;
-      unit_to_tile<EPI>(p, u, m, n, s);
+      units.tile(p, u, m, n, s);
       split_range(s, k0, k1);
       const int row = m * kTileM + static_cast<int>(rank) * kHalf;
       const int col = n * kTileN + static_cast<int>(rank) * kHalf;
       for (int kb = k0; kb < k1 && ok; ++kb) {
+        const int k = kb * kBlockK;
         for (int pr = 0; pr < (SEG ? 6 : 1); ++pr, ++step) {
           const int st = step % kStages;
           if (step >= kStages && !wait_pair_warp(&bar_empty[st], (step / kStages - 1) & 1u, s_abort)) {
             ok = false;
             break;
           }
-          const uint32_t bar = map_to_rank(smem_u32(&bar_full[st]), 0);
           if (rank == 0) mbar_expect_tx_if(leader, &bar_full[st], 2 * kStageBytes);
           uint8_t* a = smem + st * kStageBytes;
-          uint8_t* b = a + kOperandBytes;
+          const uint32_t bar = map_to_rank(smem_u32(&bar_full[st]), 0);
           const int pa = SEG ? static_cast<int>((kPlaneA >> (2 * pr)) & 3u) : 0;
-          const int pb = SEG ? static_cast<int>((kPlaneB >> (2 * pr)) & 3u) : 0;
-          const int k = kb * kBlockK;
           if (A_MN) {
             load_box_if(leader, a, &maps.a, bar, row, k, pa);
             load_box_if(leader, a + kOperandBytes / 2, &maps.a, bar, row + 64, k, pa);
           } else {
             load_box_if(leader, a, &maps.a, bar, k, row, pa);
           }
+          uint8_t* b = a + kOperandBytes;
+          const int pb = SEG ? static_cast<int>((kPlaneB >> (2 * pr)) & 3u) : 0;
           if (B_MN) {
             load_box_if(leader, b, &maps.b, bar, col, k, pb);
             load_box_if(leader, b + kOperandBytes / 2, &maps.b, bar, col + 64, k, pb);
@@ -353,9 +504,9 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
       constexpr uint32_t kStepB = B_MN ? 2048u : 32u;
       int step = 0, it = 0;                                 // blocks and accumulators so far
       bool ok = true;
-      for (int u = pair_id; u < units && ok; u += n_pairs) {
+      for (int u = units.begin; u < units.end && ok; u += units.step) {
         int m, n, s, k0, k1;
-        unit_to_tile<EPI>(p, u, m, n, s);
+        units.tile(p, u, m, n, s);
         split_range(s, k0, k1);
         const int total = (k1 - k0) * (SEG ? 6 : 1);
         const int per_segment = SEG ? kSegmentSteps : total;
@@ -375,8 +526,9 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
             }
             tc_fence_after();
             const uint32_t a = smem_u32(smem + st * kStageBytes);
+            const uint32_t b = a + kOperandBytes;
             const uint64_t da = smem_desc(a, A_MN ? kOperandBytes / 2 : 16, 1024);
-            const uint64_t db = smem_desc(a + kOperandBytes, B_MN ? kOperandBytes / 2 : 16, 1024);
+            const uint64_t db = smem_desc(b, B_MN ? kOperandBytes / 2 : 16, 1024);
 #pragma unroll
             for (int kk = 0; kk < kBlockK / 16; ++kk) {
               mma_pair_if(leader, acc, desc_add(da, kk * kStepA), desc_add(db, kk * kStepB), idesc, (i > 0 || kk > 0) ? 1u : 0u);
@@ -392,10 +544,15 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
     const int group = warp >> 2;
     const int gt = tid & (kGroupThreads - 1);
     const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    constexpr int kCols = SEG ? 128 : 256;                  // columns of a tile this group works on
-    const int c0 = SEG ? group * kCols : 0;
-    float* s_bias = reinterpret_cast<float*>(smem + kOffBias) + group * kTileN;
-    uint8_t* stage = smem + kOffStore + group * 2 * kStoreBytes;
+    constexpr int kCols = kTileN / kParts;                  // columns of a tile this group works on
+    constexpr int kBuffers = 4 / kGroups;                   // staging buffers of a group that stores by TMA
+    const int part = group % kParts;
+    const int c0 = part * kCols;
+    static_assert(kGroups * kCols * 4 <= kBiasBytes, "biases exceed their place");
+    float* s_bias = reinterpret_cast<float*>(smem + kOffBias) + group * kCols;
+    uint8_t* stage = smem + kOffStore + group * kBuffers * kStoreBytes;
+    static_assert(EPI != kEpiStore || kGroups * kBuffers * kStoreBytes <= 4 * kStoreBytes, "staging exceeds its place");
+    static_assert(EPI != kEpiGrad || 4 * kGroups * 2048 <= 4 * kStoreBytes, "staging exceeds its place");
     const int bar_id = 1 + group;
     const uint32_t free_addr[2] = {map_to_rank(smem_u32(&bar_acc_free[0]), 0), map_to_rank(smem_u32(&bar_acc_free[1]), 0)};
     int it = 0, boxes = 0;
@@ -408,9 +565,9 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
     // one 128-byte wide box of 128 rows leaves through the staging buffers: begin (the buffer is free for all
     // threads of the group) -> 16-byte pieces -> end (the store is on its way)
     auto box_begin = [&]() -> uint8_t* {
-      if (gt == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+      if (gt == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kBuffers - 1) : "memory");
       group_sync(bar_id);
-      return stage + (boxes & 1) * kStoreBytes + gt * 128;
+      return stage + (boxes % kBuffers) * kStoreBytes + gt * 128;
     };
     auto put16 = [&](uint8_t* row_ptr, int piece, uint4 v) {
       *reinterpret_cast<uint4*>(row_ptr + ((piece ^ (gt & 7)) << 4)) = v;
@@ -419,18 +576,18 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
       fence_proxy_async();
       group_sync(bar_id);
       if (gt == 0 && y < p.rows) {                           // a box wholly below the matrix is not sent
-        store_box(stage + (boxes & 1) * kStoreBytes, &maps.c, x, y, z, add);
+        store_box(stage + (boxes % kBuffers) * kStoreBytes, &maps.c, x, y, z, add);
         bulk_commit();
       }
       ++boxes;
     };
 
-    for (int u = pair_id, tile_no = 0; u < units && ok; u += n_pairs, ++tile_no) {
+    for (int u = units.begin, tile_no = 0; u < units.end && ok; u += units.step, ++tile_no) {
       int m, n, s, k0, k1;
-      unit_to_tile<EPI>(p, u, m, n, s);
+      units.tile(p, u, m, n, s);
       split_range(s, k0, k1);
       const int segments = SEG ? ((k1 - k0) * 6 + kSegmentSteps - 1) / kSegmentSteps : 1;
-      if (!SEG && (tile_no & 1) != group) {
+      if (!SEG && (tile_no & 1) != group / kParts) {
         ++it;
         continue;
       }
@@ -443,48 +600,37 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
         if (p.scale != nullptr) scale = *p.scale;
         if (p.scale2 != nullptr) scale *= *p.scale2;
       }
-      int target_col = -1;                                   // the target's column in this tile
-      float top = 0.0f, coef = 0.0f, g = 0.0f;
+      int target_col = -1;                                   // kEpiLse: the target's column among this group's
+      RowTerms terms{};
       if (EPI != kEpiStore) {
         group_sync(bar_id);                                  // everyone is done with the previous tile's s_bias
-        for (int j = gt; j < kTileN; j += kGroupThreads) {
-          const int64_t v = p.v0 + static_cast<int64_t>(n) * kTileN + j;
-          float b = -INFINITY;                               // no such word
-          if (v < p.vocab) {
-            b = 0.0f;
-            if (p.bias != nullptr) {
-              b = p.bias_dtype == GRMX_F32 ? static_cast<const float*>(p.bias)[v]
-                                           : __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[v]);
-            }
-          }
-          s_bias[j] = b * kLog2e;
-        }
-        if (live) {
-          const int64_t t = p.targets[row];
-          const bool counts = t != p.ignore_index && t >= 0 && t < p.vocab;
-          const int64_t rel = t - p.v0 - static_cast<int64_t>(n) * kTileN;
-          if (counts && rel >= 0 && rel < kTileN) target_col = static_cast<int>(rel);
-          if (EPI == kEpiGrad && counts) {
-            g = p.grad != nullptr ? p.grad[row] : 1.0f;
-            top = p.row_max[row];
-            coef = g / p.row_sum[row];
-          }
+        const int64_t first_word = p.v0 + static_cast<int64_t>(n) * kTileN + c0;
+        load_bias(p, s_bias, first_word, kCols, gt, kGroupThreads);
+        if (EPI == kEpiGrad) terms = row_terms(p, row, first_word);
+        if (EPI == kEpiLse && live) {
+          const int64_t rel = __ldg(p.targets + row) - first_word;
+          if (rel >= 0 && rel < kCols && __ldg(p.targets + row) != p.ignore_index) target_col = static_cast<int>(rel);
         }
       }
       // ---- the accumulator: streamed from TMEM, or drained segment by segment into registers
       float acc[SEG ? kCols : 1];
       if (SEG) {
+#pragma unroll
+        for (int j = 0; j < kCols; ++j) acc[SEG ? j : 0] = 0.0f;
         for (int sg = 0; sg < segments; ++sg, ++it) {
           ok = group_all(bar_id, wait_pair(&bar_acc_ready[it & 1], (it / 2) & 1u, s_abort));
           if (!ok) break;
           tc_fence_after();
 #pragma unroll
-          for (int c = 0; c < kCols; c += 32) {
-            uint32_t v[32];
-            tc_ld32_async(lane_addr + kTileN * (it & 1) + c0 + c, v);
+          for (int c = 0; c < kCols; c += 16) {              // 16 at a time: the accumulators take most of the registers
+            uint32_t v[16];
+            tc_ld16_async(lane_addr + kTileN * (it & 1) + c0 + c, v);
             tc_wait_ld();
 #pragma unroll
-            for (int j = 0; j < 32; ++j) acc[(SEG ? c : 0) + (SEG ? j : 0)] = (sg == 0 ? 0.0f : acc[(SEG ? c : 0) + (SEG ? j : 0)]) + __uint_as_float(v[j]);
+            for (int j = 0; j < 16; ++j) {
+              float& a = acc[SEG ? c + j : 0];
+              a += __uint_as_float(v[j]);
+            }
           }
           release(it & 1);
         }
@@ -494,7 +640,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
       }
       if (!ok) break;
       // (group_all above also made s_bias visible to the group)
-      const uint32_t acc_addr = lane_addr + kTileN * (it & 1);
+      const uint32_t acc_addr = lane_addr + kTileN * (it & 1) + c0;
       auto fetch = [&](int c, float (&v)[32]) {              // columns [c, c + 32) of this group's part
         if (SEG) {
 #pragma unroll
@@ -509,128 +655,127 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
       };
 
       if (EPI == kEpiLse) {
-        // running maximum and sum over the columns, base 2: y = score * log2 e + bias * log2 e
+        // running maximum and sum over the columns, base 2
         float mx = -INFINITY, sum = 0.0f;
 #pragma unroll
         for (int c = 0; c < kCols; c += 32) {
           float y[32];
           fetch(c, y);
-          float best = -INFINITY;
+          scores_base2(y, s_bias + c);
+          float best[4] = {y[0], y[1], y[2], y[3]};
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            y[j] = fmaf(y[j], kLog2e, s_bias[c0 + c + j]);
-            best = fmaxf(best, y[j]);
-          }
-          const int hit = target_col - c0 - c;
+          for (int j = 4; j < 32; ++j) best[j & 3] = fmaxf(best[j & 3], y[j]);
+          const int hit = target_col - c;
           if (__any_sync(0xffffffffu, hit >= 0 && hit < 32)) {
 #pragma unroll
             for (int j = 0; j < 32; ++j) {
               if (hit == j) p.target_score[row] = y[j];
             }
           }
-          const float next = fmaxf(mx, best);
+          const float next = fmaxf(fmaxf(mx, fmaxf(best[0], best[1])), fmaxf(best[2], best[3]));
           const float base = next == -INFINITY ? 0.0f : next;   // nothing finite so far: every term is 2^-inf = 0
-          float part = 0.0f;
+          const uint64_t shift = pack2(-base, -base);
+          uint64_t part[2] = {0ull, 0ull};
 #pragma unroll
-          for (int j = 0; j < 32; ++j) part += exp2_fast(y[j] - base);
-          sum = sum * exp2_fast(mx - base) + part;
+          for (int j = 0; j < 32; j += 2) {
+            float lo, hi;
+            unpack2(add2(pack2(y[j], y[j + 1]), shift), lo, hi);
+            part[(j >> 1) & 1] = add2(part[(j >> 1) & 1], pack2(exp2_fast(lo), exp2_fast(hi)));
+          }
+          float lo, hi;
+          unpack2(add2(part[0], part[1]), lo, hi);
+          sum = fmaf(sum, exp2_fast(mx - base), lo + hi);
           mx = next;
         }
         if (!SEG) release(it & 1);
         if (live) {
-          const int64_t part = SEG ? 2 * static_cast<int64_t>(n) + group : n;
-          p.partials[part * p.rows + row] = make_float2(mx, sum);
+          p.partials[(static_cast<int64_t>(n) * kParts + part) * p.rows + row] = make_float2(mx, sum);
         }
-      } else if (EPI == kEpiGrad) {
-        // d = g * (2^(y - top) / sum - [target]); ignored rows have g = coef = 0 and are written as zeros
-        const bool counts = coef != 0.0f || g != 0.0f;
-        constexpr int nplanes = SEG ? 3 : 1;
+      } else if constexpr (EPI == kEpiGrad) {
+        // Every warp stages and sends its own 32 rows, 32 columns at a time; no barrier between warps.
+        uint8_t* box = smem + kOffStore + warp * 2048;
+        const int64_t first_col = static_cast<int64_t>(n) * kTileN + c0;
+        const int rows_here = static_cast<int>(max(int64_t(0), min(int64_t(32), p.rows - row + lane)));
+        __nv_bfloat16* out = p.d_out + (row - lane) * p.d_ld + first_col;
+        // column sums: one row of them per 32 token rows, added up by a kernel of its own
+        float* col_sums = p.bias_partials + (static_cast<int64_t>(m) * 8 + rank * 4 + (warp & 3)) * (static_cast<int64_t>(p.n_tiles) * kTileN) + first_col;
 #pragma unroll
-        for (int c = 0; c < kCols; c += 64) {
-          float d[64];
+        for (int c = 0; c < kCols; c += 32) {
+          float d[32];
+          fetch(c, d);
+          if (!SEG && c + 32 == kCols) release(it & 1);
+          score_gradient(d, s_bias + c, terms, c);
+          if (SEG && p.bias_partials != nullptr) {
+            float v[32];
 #pragma unroll
-          for (int h = 0; h < 64; h += 32) {
-            float y[32];
-            fetch(c + h, y);
-#pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              const float e = exp2_fast(fmaf(y[j], kLog2e, s_bias[c0 + c + h + j]) - top);
-              d[h + j] = counts ? e * coef : 0.0f;
-            }
-            const int hit = target_col - c0 - c - h;
-            if (__any_sync(0xffffffffu, hit >= 0 && hit < 32)) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j) {
-                if (hit == j) d[h + j] -= g;
-              }
-            }
-            if (p.bias_partials != nullptr) {
-              float v[32];
-#pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = d[h + j];
-              const float total = transpose_sum(v, lane);
-              // one row of sums per 32 token rows; the reduction over them follows in a kernel of its own
-              const int64_t block = static_cast<int64_t>(m) * 8 + rank * 4 + (warp & 3);
-              p.bias_partials[block * (static_cast<int64_t>(p.n_tiles) * kTileN) + static_cast<int64_t>(n) * kTileN + c0 + c + h + lane] = total;
-            }
+            for (int j = 0; j < 32; ++j) v[j] = d[j];
+            col_sums[c + lane] = transpose_sum(v, lane);
           }
-          if (!SEG && c + 64 == kCols) release(it & 1);
 #pragma unroll
-          for (int pl = 0; pl < nplanes; ++pl) {
-            uint8_t* dst = box_begin();
+          for (int pl = 0; pl < (SEG ? 3 : 1); ++pl) {
 #pragma unroll
-            for (int q = 0; q < 8; ++q) {
+            for (int q = 0; q < 4; ++q) {
               uint32_t w[4];
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                const int j = 8 * q + 2 * e;
-                w[e] = pack_bf16(d[j], d[j + 1]);
+                float& lo = d[8 * q + 2 * e];
+                float& hi = d[8 * q + 2 * e + 1];
+                w[e] = pack_bf16(lo, hi);
                 if (SEG) {
                   const __nv_bfloat162 b = *reinterpret_cast<const __nv_bfloat162*>(&w[e]);
-                  d[j] -= __low2float(b);
-                  d[j + 1] -= __high2float(b);
+                  lo -= __low2float(b);
+                  hi -= __high2float(b);
                 }
               }
-              put16(dst, q, make_uint4(w[0], w[1], w[2], w[3]));
+              *reinterpret_cast<uint4*>(box_piece(box, lane, q)) = make_uint4(w[0], w[1], w[2], w[3]);
             }
-            box_end(n * kTileN + c0 + c, row0, pl, false);
+            __syncwarp();
+            __nv_bfloat16* dst = out + c + pl * p.d_plane_stride;
+            if (!SEG && p.bias_partials != nullptr) {
+              // sums of the rounded values, which is what the weights' gradient is made of as well
+              const float2 sums = box_out<true>(box, dst, p.d_ld, rows_here, lane);
+              if ((lane & 4) == 0) *reinterpret_cast<float2*>(col_sums + c + box_column(lane)) = sums;
+            } else {
+              box_out<false>(box, dst, p.d_ld, rows_here, lane);
+            }
+            __syncwarp();
           }
         }
       } else {
         // plain result: fp32 boxes of 32 columns or bf16 boxes of 64; rows and columns beyond the matrix are
         // clipped by the store, boxes wholly beyond it are not sent
         const int limit = static_cast<int>(min(p.cols - static_cast<int64_t>(n) * kTileN, static_cast<int64_t>(kTileN)));
+        if (p.store_f32) {
 #pragma unroll
-        for (int c = 0; c < kCols; c += 64) {
-          float d[64];
-#pragma unroll
-          for (int h = 0; h < 64; h += 32) {
-            float y[32];
-            fetch(c + h, y);
-#pragma unroll
-            for (int j = 0; j < 32; ++j) d[h + j] = y[j] * scale;
-          }
-          if (!SEG && c + 64 == kCols) release(it & 1);
-          if (c0 + c >= limit) continue;
-          if (p.store_f32) {
-#pragma unroll
-            for (int h = 0; h < 64; h += 32) {
-              if (c0 + c + h >= limit) continue;
-              uint8_t* dst = box_begin();
-#pragma unroll
-              for (int q = 0; q < 8; ++q) {
-                put16(dst, q, make_uint4(__float_as_uint(d[h + 4 * q]), __float_as_uint(d[h + 4 * q + 1]),
-                                         __float_as_uint(d[h + 4 * q + 2]), __float_as_uint(d[h + 4 * q + 3])));
-              }
-              box_end(n * kTileN + c0 + c + h, row0, s, p.store_add != 0);
-            }
-          } else {
+          for (int c = 0; c < kCols; c += 32) {
+            float d[32];
+            fetch(c, d);
+            if (!SEG && c + 32 == kCols) release(it & 1);
+            if (c0 + c >= limit) continue;
             uint8_t* dst = box_begin();
 #pragma unroll
             for (int q = 0; q < 8; ++q) {
-              put16(dst, q, make_uint4(pack_bf16(d[8 * q], d[8 * q + 1]), pack_bf16(d[8 * q + 2], d[8 * q + 3]),
-                                       pack_bf16(d[8 * q + 4], d[8 * q + 5]), pack_bf16(d[8 * q + 6], d[8 * q + 7])));
+              put16(dst, q, make_uint4(__float_as_uint(d[4 * q] * scale), __float_as_uint(d[4 * q + 1] * scale),
+                                       __float_as_uint(d[4 * q + 2] * scale), __float_as_uint(d[4 * q + 3] * scale)));
             }
+            box_end(n * kTileN + c0 + c, row0, s, p.store_add != 0);
+          }
+        } else if constexpr (!SEG) {                         // full precision has no bf16 results
+#pragma unroll
+          for (int c = 0; c < kCols; c += 64) {
+            uint32_t w[32];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              float d[32];
+              fetch(c + 32 * h, d);
+#pragma unroll
+              for (int j = 0; j < 16; ++j) w[16 * h + j] = pack_bf16(d[2 * j] * scale, d[2 * j + 1] * scale);
+            }
+            if (c + 64 == kCols) release(it & 1);
+            if (c0 + c >= limit) continue;
+            uint8_t* dst = box_begin();
+#pragma unroll
+            for (int q = 0; q < 8; ++q) put16(dst, q, make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]));
             box_end(n * kTileN + c0 + c, row0, s, false);
           }
         }
