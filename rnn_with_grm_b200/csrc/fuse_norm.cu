@@ -12,17 +12,19 @@
 // (the reference runs these as separate ATen calls: grm/core/aggregator.py:116-145 for the rules,
 // grm/core/multilayer_grm.py:93,96 for the residual block between layers.)
 //
-// Bound by memory: every row tensor crosses once.  A row belongs to 32, 128 or 512 threads, at most 16 values
-// each, so that a row, and in the backward pass the column sums of all rows a thread has seen, stay in
-// registers; mean and variance are two passes over those registers.  Row sums are fp32; column sums are fp32
-// per thread, then joined in a fixed order (groups of a CTA in shared memory, CTAs by a second kernel).
+// Bound by memory: every row tensor crosses once.  A row belongs to 32 ... 1024 threads, at most 16 values each forward
+// and 8 backward, so that a row, and in the backward pass the column sums of all rows a thread has seen, stay in registers
+// with enough warps resident to cover the loads (backward with 16 values: one CTA per SM, 157 us for 65536 x 512 bf16 against
+// 121 with 8); mean and variance are two passes over those registers.  Row sums are fp32; column sums are fp32 per
+// thread, then joined in a fixed order (groups of a CTA in shared memory, CTAs by a second kernel).
 #include "common.cuh"
 
 namespace grmx {
 namespace {
 
-constexpr int kPerThread = 16;
-constexpr int kMaxWidth = 512 * kPerThread;
+// values of a row per thread
+constexpr int kForward = 16, kBackward = 8;
+constexpr int kMaxWidth = 1024 * kBackward;
 
 struct RowArgs {
   const void *online, *update, *gate;     // [rows, H]; gate may be NULL
@@ -35,6 +37,7 @@ struct RowArgs {
   float* col_partials;                    // backward: [kinds][CTAs][H]
   int64_t rows;
   int H;
+  int param_bf16;                         // scale, weight and bias are bf16, not fp32
   int want_scale, want_weight, want_bias;
 };
 
@@ -44,18 +47,26 @@ template <typename T>
 struct Raw<T, 1> {
   T v;
   __device__ __forceinline__ void load(const T* p) { v = __ldg(p); }
+  __device__ __forceinline__ void set(const T (&x)[1]) { v = x[0]; }
   __device__ __forceinline__ void unpack(float (&x)[1]) const { x[0] = to_float<T>(v); }
 };
 template <>
 struct Raw<float, 4> {
   float4 v;
   __device__ __forceinline__ void load(const float* p) { v = __ldg(reinterpret_cast<const float4*>(p)); }
+  __device__ __forceinline__ void set(const float (&x)[4]) { v = make_float4(x[0], x[1], x[2], x[3]); }
   __device__ __forceinline__ void unpack(float (&x)[4]) const { x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w; }
 };
 template <>
 struct Raw<__nv_bfloat16, 8> {
   uint4 v;
   __device__ __forceinline__ void load(const __nv_bfloat16* p) { v = __ldg(reinterpret_cast<const uint4*>(p)); }
+  __device__ __forceinline__ void set(const __nv_bfloat16 (&x)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = static_cast<uint32_t>(__bfloat16_as_ushort(x[2 * i])) | (static_cast<uint32_t>(__bfloat16_as_ushort(x[2 * i + 1])) << 16);
+    v = make_uint4(w[0], w[1], w[2], w[3]);
+  }
   __device__ __forceinline__ void unpack(float (&x)[8]) const {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -80,110 +91,208 @@ __device__ __forceinline__ void store_vec(__nv_bfloat16* p, const float (&x)[8])
   *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// sigmoid(g) and 1 - sigmoid(g), both to full relative precision
+// sigmoid(g) and 1 - sigmoid(g), both to full relative precision: with t = exp(-|g|) they are 1 / (1 + t) and t / (1 + t)
 __device__ __forceinline__ void sigmoid_pair(float g, float& yes, float& no) {
-  const float t = __expf(-fabsf(g));
-  const float r = __fdividef(1.0f, 1.0f + t);
+  float t, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(fabsf(g) * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + t));
   const float small = t * r;
   yes = g >= 0.0f ? r : small;
   no = g >= 0.0f ? small : r;
-  if (isnan(g)) yes = no = g;
 }
 
-// sums over the G threads of a row; all of them get the result
+// Sums over the G threads of a row; all of them get the result.  `turn` alternates between two places for the warps'
+// parts: whoever writes to one of them has passed the barrier that followed the last read of it.
 template <int G>
-__device__ __forceinline__ float2 row_sum2(float2 v, float2* scratch) {
+__device__ __forceinline__ float2 row_sum2(float2 v, float2 (*scratch)[G / 32], int& turn) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
     v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
   }
   if (G > 32) {
-    constexpr int kWarps = G / 32;
-    const int warp = (threadIdx.x % G) >> 5;
-    const int id = 1 + threadIdx.x / G;
-    asm volatile("barrier.cta.sync %0, %1;" ::"r"(id), "n"(G) : "memory");       // the scratch of the last sum has been read
-    if ((threadIdx.x & 31) == 0) scratch[warp] = v;
-    asm volatile("barrier.cta.sync %0, %1;" ::"r"(id), "n"(G) : "memory");
+    float2* parts = scratch[turn];
+    turn ^= 1;
+    if ((threadIdx.x & 31) == 0) parts[(threadIdx.x % G) >> 5] = v;
+    asm volatile("barrier.cta.sync %0, %1;" ::"r"(1 + static_cast<int>(threadIdx.x) / G), "n"(G) : "memory");
     v = make_float2(0.0f, 0.0f);
 #pragma unroll
-    for (int i = 0; i < kWarps; ++i) {
-      v.x += scratch[i].x;
-      v.y += scratch[i].y;
+    for (int i = 0; i < G / 32; ++i) {
+      v.x += parts[i].x;
+      v.y += parts[i].y;
     }
   }
   return v;
 }
 
-template <typename P, int VEC>
-__device__ __forceinline__ void load_param(const void* base, int h, float fill, float (&x)[VEC]) {
-  if (base == nullptr) {
+template <int G>
+__device__ __forceinline__ float row_sum(float v, float2 (*scratch)[G / 32], int& turn) {
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) x[j] = fill;
-    return;
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if (G > 32) {
+    float2* parts = scratch[turn];
+    turn ^= 1;
+    if ((threadIdx.x & 31) == 0) parts[(threadIdx.x % G) >> 5].x = v;
+    asm volatile("barrier.cta.sync %0, %1;" ::"r"(1 + static_cast<int>(threadIdx.x) / G), "n"(G) : "memory");
+    v = 0.0f;
+#pragma unroll
+    for (int i = 0; i < G / 32; ++i) v += parts[i].x;
   }
-  const P* p = static_cast<const P*>(base) + h;
-  if constexpr (VEC == 1) {
-    x[0] = to_float<P>(__ldg(p));
-  } else if constexpr (sizeof(P) == 4) {
-#pragma unroll
-    for (int j = 0; j < VEC; j += 4) {
-      const float4 q = __ldg(reinterpret_cast<const float4*>(p + j));
-      x[j] = q.x; x[j + 1] = q.y; x[j + 2] = q.z; x[j + 3] = q.w;
-    }
-  } else {
-    Raw<P, VEC> raw;
+  return v;
+}
+
+__host__ __device__ constexpr int threads_of(int G) { return G > 256 ? G : 256; }
+
+// How a thread sees the rows it works on.
+//
+//   kWhole   rows start on 16-byte boundaries: pieces of VEC values (16 bytes)
+//   kShifted rows of any width in tensors that start on a 16-byte boundary: the same 16-byte pieces of memory, so a row begins
+//            `off` values into its first piece and its pieces' columns are shifted by that.  off = row * H mod VEC is the
+//            same for all rows of a thread because the number of row groups of a launch is a multiple of VEC.  Pieces that
+//            stick out of the row are stored value by value, the one that sticks out of the tensor is read so.
+//   kSingle  tensors that start anywhere: value by value (VEC = 1)
+//
+// Piece i < count (the same for all threads of the row) starts at column at(i).  With whole pieces and single values the
+// last piece of a thread may lie behind the row: it reads the row's last columns instead and does not count.
+enum Access { kWhole, kShifted, kSingle };
+
+template <int VEC, int G, int ACCESS>
+struct Columns {
+  int H, off, count, first;
+  __device__ __forceinline__ Columns(int width, int64_t first_row, int lane) : H(width) {
+    off = ACCESS == kShifted ? static_cast<int>((first_row * H) % VEC) : 0;
+    count = (H + off + G * VEC - 1) / (G * VEC);
+    first = lane * VEC - off;
+  }
+  __device__ __forceinline__ int start(int i) const { return first + G * VEC * i; }
+  // any of the piece's values belongs to the row
+  __device__ __forceinline__ bool live(int i) const { return start(i) < H; }
+  __device__ __forceinline__ int at(int i) const { return ACCESS == kShifted ? start(i) : min(start(i), H - VEC); }
+  __device__ __forceinline__ bool holds(int c) const { return ACCESS != kShifted || (c >= 0 && c < H); }
+  __device__ __forceinline__ bool inside(int i) const { return ACCESS != kShifted || (start(i) >= 0 && start(i) + VEC <= H); }
+};
+
+template <typename T, int VEC, int ACCESS>
+__device__ __forceinline__ void load_piece(Raw<T, VEC>& raw, const void* tensor, int64_t base, int c, bool live, int64_t total) {
+  const T* p = static_cast<const T*>(tensor) + base + c;
+  if (ACCESS != kShifted) {
     raw.load(p);
-    raw.unpack(x);
+  } else if (live && base + c + VEC <= total) {
+    raw.load(p);
+  } else {
+    T v[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) v[j] = live && base + c + j < total ? __ldg(p + j) : from_float<T>(0.0f);
+    raw.set(v);
+  }
+}
+template <typename T, int VEC, int ACCESS, int G>
+__device__ __forceinline__ void store_piece(void* tensor, int64_t base, const Columns<VEC, G, ACCESS>& col, int i, const float (&x)[VEC]) {
+  if (!col.live(i)) return;
+  T* p = static_cast<T*>(tensor) + base + col.at(i);
+  if (col.inside(i)) {
+    store_vec(p, x);
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      if (col.holds(col.at(i) + j)) p[j] = from_float<T>(x[j]);
+    }
   }
 }
 
-__host__ __device__ constexpr int threads_of(int G) { return G == 512 ? 512 : 256; }
+// Parameters of a piece's columns.  Shifted rows take them from shared memory (fp32, one word of padding after every
+// eight, so that the 32 lanes' reads at a distance of a piece do not collide).
+__device__ __forceinline__ int padded(int c) { return c + (c >> 3); }
+// (Volatile reads: the values are the same for all rows of a thread, and a compiler that keeps them in registers from row
+// to row spills others.)
+__device__ __forceinline__ uint4 load_again(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+template <int VEC, int ACCESS>
+__device__ __forceinline__ void load_param(const RowArgs& a, const void* base, const float* staged, int c, float fill, float (&x)[VEC]) {
+  if (base == nullptr) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) x[j] = fill;
+  } else if (ACCESS == kShifted) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) x[j] = static_cast<const volatile float*>(staged)[padded(max(0, min(c + j, a.H - 1)))];
+  } else if (a.param_bf16) {
+    const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(base) + c;
+    if constexpr (VEC == 8) {
+      Raw<__nv_bfloat16, 8> raw;
+      raw.v = load_again(p);
+      raw.unpack(x);
+    } else {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) x[j] = __bfloat162float(__ldg(p + j));
+    }
+  } else {
+    const float* p = static_cast<const float*>(base) + c;
+    if constexpr (VEC % 4 == 0) {
+#pragma unroll
+      for (int j = 0; j < VEC; j += 4) {
+        const uint4 q = load_again(p + j);
+        x[j] = __uint_as_float(q.x); x[j + 1] = __uint_as_float(q.y); x[j + 2] = __uint_as_float(q.z); x[j + 3] = __uint_as_float(q.w);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) x[j] = __ldg(p + j);
+    }
+  }
+}
+__device__ __forceinline__ void stage_params(const RowArgs& a, float* dst, const void* base, int threads) {
+  if (base == nullptr) return;
+  for (int c = threadIdx.x; c < a.H; c += threads) {
+    dst[padded(c)] = a.param_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(base)[c]) : static_cast<const float*>(base)[c];
+  }
+}
+__host__ __device__ constexpr int staged_words(int H) { return H + H / 8 + 1; }
 
-// The columns of a row that a thread holds: pieces i < count (the same count for all threads), piece i at column
-// (lane + G i) VEC.  The last piece may lie behind the row: its loads go to the row's last columns instead (always
-// in bounds), its values count as zero and are not stored.
-template <int VEC, int G>
-struct Columns {
-  int count, first, last;      // last: the largest column a piece can start at
-  __device__ __forceinline__ Columns(int H, int lane) : count((H + G * VEC - 1) / (G * VEC)), first(lane * VEC), last(H - VEC) {}
-  __device__ __forceinline__ int at(int i) const { return min(first + G * VEC * i, last); }
-  __device__ __forceinline__ bool live(int i) const { return first + G * VEC * i <= last; }
-};
-
-template <typename T, typename P, int VEC, int G, bool GATE>
-__global__ void __launch_bounds__(threads_of(G))
+template <typename T, int VEC, int G, int ACCESS, bool GATE>
+__global__ void __launch_bounds__(threads_of(G), G > 256 ? 1 : 3)
 fuse_norm_fwd_kernel(const __grid_constant__ RowArgs a) {
-  constexpr int kPieces = kPerThread / VEC;
+  constexpr int kPieces = kForward / VEC;
   constexpr int kGroups = threads_of(G) / G;
-  __shared__ float2 s_scratch[kGroups][G / 32];
+  __shared__ float2 s_scratch[kGroups][2][G / 32];
+  int turn = 0;
+  extern __shared__ float s_params[];                    // shifted rows: weight, bias, scale
   const int group = threadIdx.x / G, lane = threadIdx.x % G;
   const int H = a.H;
-  const Columns<VEC, G> col(H, lane);
+  const float *p_weight = s_params, *p_bias = s_params + staged_words(H), *p_scale = s_params + 2 * staged_words(H);
+  if (ACCESS == kShifted) {
+    stage_params(a, s_params, a.weight, threads_of(G));
+    stage_params(a, s_params + staged_words(H), a.bias, threads_of(G));
+    stage_params(a, s_params + 2 * staged_words(H), a.scale, threads_of(G));
+    __syncthreads();
+  }
+  const int64_t first_row = static_cast<int64_t>(blockIdx.x) * kGroups + group, total = a.rows * H;
+  const Columns<VEC, G, ACCESS> col(H, first_row, lane);
   const float inv = 1.0f / static_cast<float>(H);
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * kGroups + group; row < a.rows; row += static_cast<int64_t>(gridDim.x) * kGroups) {
+#pragma unroll 1
+  for (int64_t row = first_row; row < a.rows; row += static_cast<int64_t>(gridDim.x) * kGroups) {
     const int64_t base = row * H;
     Raw<T, VEC> ro[kPieces], ru[kPieces], rg[kPieces];
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
       if (i < col.count) {
-        ro[i].load(static_cast<const T*>(a.online) + base + col.at(i));
-        ru[i].load(static_cast<const T*>(a.update) + base + col.at(i));
-        if (GATE) rg[i].load(static_cast<const T*>(a.gate) + base + col.at(i));
+        load_piece<T, VEC, ACCESS>(ro[i], a.online, base, col.at(i), col.live(i), total);
+        load_piece<T, VEC, ACCESS>(ru[i], a.update, base, col.at(i), col.live(i), total);
+        if (GATE) load_piece<T, VEC, ACCESS>(rg[i], a.gate, base, col.at(i), col.live(i), total);
       }
     }
     float s[kPieces][VEC];
-    float2 sum = make_float2(0.0f, 0.0f);
+    float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
       if (i < col.count) {
-        const int h = col.at(i);
         const bool live = col.live(i);
         float o[VEC], u[VEC], k[VEC];
         ro[i].unpack(o);
         ru[i].unpack(u);
         if (a.scale != nullptr) {
-          load_param<P, VEC>(a.scale, h, 1.0f, k);
+          load_param<VEC, ACCESS>(a, a.scale, p_scale, col.at(i), 1.0f, k);
 #pragma unroll
           for (int j = 0; j < VEC; ++j) u[j] *= k[j];
         }
@@ -197,50 +306,57 @@ fuse_norm_fwd_kernel(const __grid_constant__ RowArgs a) {
           } else {
             s[i][j] = o[j] + u[j];
           }
-          if (live) sum.x += s[i][j];
+          if (live && col.holds(col.at(i) + j)) sum += s[i][j];
         }
-        if (a.sum_out != nullptr && live) store_vec(static_cast<T*>(a.sum_out) + base + h, s[i]);
+        if (a.sum_out != nullptr) store_piece<T>(a.sum_out, base, col, i, s[i]);
       }
     }
-    const float mean = row_sum2<G>(sum, s_scratch[group]).x * inv;
-    sum = make_float2(0.0f, 0.0f);
+    const float mean = row_sum<G>(sum, s_scratch[group], turn) * inv;
+    sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
       if (i < col.count && col.live(i)) {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
           const float d = s[i][j] - mean;
-          sum.x = fmaf(d, d, sum.x);
+          if (col.holds(col.at(i) + j)) sum = fmaf(d, d, sum);
         }
       }
     }
-    const float rstd = rsqrtf(row_sum2<G>(sum, s_scratch[group]).x * inv + a.eps);
+    const float rstd = rsqrtf(row_sum<G>(sum, s_scratch[group], turn) * inv + a.eps);
     if (lane == 0 && a.stats != nullptr) a.stats[row] = make_float2(mean, rstd);
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
       if (i < col.count) {
-        const int h = col.at(i);
-        float w[VEC], b[VEC], y[VEC];
-        load_param<P, VEC>(a.weight, h, 1.0f, w);
-        load_param<P, VEC>(a.bias, h, 0.0f, b);
+        float w[VEC], b[VEC];
+        load_param<VEC, ACCESS>(a, a.weight, p_weight, col.at(i), 1.0f, w);
+        load_param<VEC, ACCESS>(a, a.bias, p_bias, col.at(i), 0.0f, b);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) y[j] = fmaf((s[i][j] - mean) * rstd, w[j], b[j]);
-        if (col.live(i)) store_vec(static_cast<T*>(a.out) + base + h, y);
+        for (int j = 0; j < VEC; ++j) s[i][j] = fmaf((s[i][j] - mean) * rstd, w[j], b[j]);
+        store_piece<T>(a.out, base, col, i, s[i]);
       }
     }
   }
 }
 
-template <typename T, typename P, int VEC, int G, bool GATE, bool SCALE>
-__global__ void __launch_bounds__(threads_of(G))
+template <typename T, int VEC, int G, int ACCESS, bool GATE, bool SCALE>
+__global__ void __launch_bounds__(threads_of(G), G > 256 ? 1 : 3)
 fuse_norm_bwd_kernel(const __grid_constant__ RowArgs a) {
-  constexpr int kPieces = kPerThread / VEC;
+  constexpr int kPieces = kBackward / VEC;
   constexpr int kGroups = threads_of(G) / G;
-  __shared__ float2 s_scratch[kGroups][G / 32];
-  __shared__ float s_cols[kGroups > 1 ? kGroups * G * kPerThread : 1];
+  __shared__ float2 s_scratch[kGroups][2][G / 32];
+  int turn = 0;
+  extern __shared__ float s_dynamic[];                   // shifted rows: weight, scale; then, at the end, the column sums
   const int group = threadIdx.x / G, lane = threadIdx.x % G;
   const int H = a.H;
-  const Columns<VEC, G> col(H, lane);
+  const float *p_weight = s_dynamic, *p_scale = s_dynamic + staged_words(H);
+  if (ACCESS == kShifted) {
+    stage_params(a, s_dynamic, a.weight, threads_of(G));
+    stage_params(a, s_dynamic + staged_words(H), a.scale, threads_of(G));
+    __syncthreads();
+  }
+  const int64_t first_row = static_cast<int64_t>(blockIdx.x) * kGroups + group, total = a.rows * H;
+  const Columns<VEC, G, ACCESS> col(H, first_row, lane);
   const float inv = 1.0f / static_cast<float>(H);
   float cw[kPieces][VEC], cb[kPieces][VEC], cs[SCALE ? kPieces : 1][VEC];
 #pragma unroll
@@ -248,7 +364,8 @@ fuse_norm_bwd_kernel(const __grid_constant__ RowArgs a) {
 #pragma unroll
     for (int j = 0; j < VEC; ++j) cw[i][j] = cb[i][j] = cs[SCALE ? i : 0][j] = 0.0f;
   }
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * kGroups + group; row < a.rows; row += static_cast<int64_t>(gridDim.x) * kGroups) {
+#pragma unroll 1
+  for (int64_t row = first_row; row < a.rows; row += static_cast<int64_t>(gridDim.x) * kGroups) {
     const int64_t base = row * H;
     Raw<T, VEC> rd[kPieces], ro[kPieces], ru[kPieces], rg[kPieces];
     const float2 st = __ldg(a.stats + row);
@@ -256,10 +373,10 @@ fuse_norm_bwd_kernel(const __grid_constant__ RowArgs a) {
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
       if (i < col.count) {
-        if (have_dy) rd[i].load(static_cast<const T*>(a.grad_out) + base + col.at(i));
-        ro[i].load(static_cast<const T*>(a.online) + base + col.at(i));
-        ru[i].load(static_cast<const T*>(a.update) + base + col.at(i));
-        if (GATE) rg[i].load(static_cast<const T*>(a.gate) + base + col.at(i));
+        if (have_dy) load_piece<T, VEC, ACCESS>(rd[i], a.grad_out, base, col.at(i), col.live(i), total);
+        load_piece<T, VEC, ACCESS>(ro[i], a.online, base, col.at(i), col.live(i), total);
+        load_piece<T, VEC, ACCESS>(ru[i], a.update, base, col.at(i), col.live(i), total);
+        if (GATE) load_piece<T, VEC, ACCESS>(rg[i], a.gate, base, col.at(i), col.live(i), total);
       }
     }
     float xh[kPieces][VEC], da[kPieces][VEC];
@@ -267,13 +384,12 @@ fuse_norm_bwd_kernel(const __grid_constant__ RowArgs a) {
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
       if (i < col.count) {
-        const int h = col.at(i);
         const bool live = col.live(i);
         float o[VEC], u[VEC], k[VEC], w[VEC];
         ro[i].unpack(o);
         ru[i].unpack(u);
         if (SCALE) {
-          load_param<P, VEC>(a.scale, h, 1.0f, k);
+          load_param<VEC, ACCESS>(a, a.scale, p_scale, col.at(i), 1.0f, k);
 #pragma unroll
           for (int j = 0; j < VEC; ++j) u[j] *= k[j];
         }
@@ -290,7 +406,7 @@ fuse_norm_bwd_kernel(const __grid_constant__ RowArgs a) {
           }
           xh[i][j] = (s - st.x) * st.y;
         }
-        load_param<P, VEC>(a.weight, h, 1.0f, w);
+        load_param<VEC, ACCESS>(a, a.weight, p_weight, col.at(i), 1.0f, w);
         if (have_dy) {
           rd[i].unpack(o);
         } else {
@@ -300,7 +416,7 @@ fuse_norm_bwd_kernel(const __grid_constant__ RowArgs a) {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
           da[i][j] = o[j] * w[j];
-          if (live) {
+          if (live && col.holds(col.at(i) + j)) {
             cw[i][j] = fmaf(o[j], xh[i][j], cw[i][j]);
             cb[i][j] += o[j];
             sum.x += da[i][j];
@@ -309,24 +425,23 @@ fuse_norm_bwd_kernel(const __grid_constant__ RowArgs a) {
         }
       }
     }
-    sum = row_sum2<G>(sum, s_scratch[group]);
+    sum = row_sum2<G>(sum, s_scratch[group], turn);
     const float m1 = sum.x * inv, m2 = sum.y * inv;
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
       if (i < col.count) {
-        const int h = col.at(i);
         const bool live = col.live(i);
         float ds[VEC], dv[VEC], u[VEC], k[VEC];
 #pragma unroll
         for (int j = 0; j < VEC; ++j) ds[j] = st.y * (da[i][j] - m1 - xh[i][j] * m2);
         if (a.grad_sum != nullptr) {
           Raw<T, VEC> raw;
-          raw.load(static_cast<const T*>(a.grad_sum) + base + h);
+          load_piece<T, VEC, ACCESS>(raw, a.grad_sum, base, col.at(i), live, total);
           raw.unpack(dv);
 #pragma unroll
           for (int j = 0; j < VEC; ++j) ds[j] += dv[j];
         }
-        if (SCALE) load_param<P, VEC>(a.scale, h, 1.0f, k);
+        if (SCALE) load_param<VEC, ACCESS>(a, a.scale, p_scale, col.at(i), 1.0f, k);
         ru[i].unpack(u);
         if (GATE) {
           float o[VEC], g[VEC], dg[VEC];
@@ -340,20 +455,20 @@ fuse_norm_bwd_kernel(const __grid_constant__ RowArgs a) {
             dv[j] = ds[j] * no;
             ds[j] *= yes;
           }
-          if (a.grad_gate != nullptr && live) store_vec(static_cast<T*>(a.grad_gate) + base + h, dg);
+          if (a.grad_gate != nullptr) store_piece<T>(a.grad_gate, base, col, i, dg);
         } else {
 #pragma unroll
           for (int j = 0; j < VEC; ++j) dv[j] = ds[j];
         }
-        if (a.grad_online != nullptr && live) store_vec(static_cast<T*>(a.grad_online) + base + h, ds);
+        if (a.grad_online != nullptr) store_piece<T>(a.grad_online, base, col, i, ds);
         if (SCALE) {
 #pragma unroll
           for (int j = 0; j < VEC; ++j) {
-            if (live) cs[SCALE ? i : 0][j] = fmaf(dv[j], u[j], cs[SCALE ? i : 0][j]);
+            if (live && col.holds(col.at(i) + j)) cs[SCALE ? i : 0][j] = fmaf(dv[j], u[j], cs[SCALE ? i : 0][j]);
             dv[j] *= k[j];
           }
         }
-        if (a.grad_update != nullptr && live) store_vec(static_cast<T*>(a.grad_update) + base + h, dv);
+        if (a.grad_update != nullptr) store_piece<T>(a.grad_update, base, col, i, dv);
       }
     }
   }
@@ -362,29 +477,25 @@ fuse_norm_bwd_kernel(const __grid_constant__ RowArgs a) {
   int kind = 0;
   auto emit = [&](float (&c)[kPieces][VEC]) {
     float* dst = a.col_partials + (static_cast<int64_t>(kind++) * gridDim.x + blockIdx.x) * H;
-    if (kGroups == 1) {
-#pragma unroll
-      for (int i = 0; i < kPieces; ++i) {
-        const int h = (lane + G * i) * VEC;
-        if (h < H) {
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) dst[h + j] = c[i][j];
-        }
-      }
-      return;
-    }
-    __syncthreads();
+    if (kGroups > 1) __syncthreads();                    // the parameters, or the last kind's sums, have been read
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
+      if (i < col.count && col.live(i)) {
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) s_cols[group * (G * kPerThread) + (lane + G * i) * VEC + j] = c[i][j];
+        for (int j = 0; j < VEC; ++j) {
+          const int h = col.at(i) + j;
+          if (col.holds(h)) (kGroups > 1 ? s_dynamic + group * H : dst)[h] = c[i][j];
+        }
+      }
     }
-    __syncthreads();
-    for (int h = threadIdx.x; h < H; h += threads_of(G)) {
-      float sum = 0.0f;
+    if (kGroups > 1) {
+      __syncthreads();
+      for (int h = threadIdx.x; h < H; h += threads_of(G)) {
+        float sum = 0.0f;
 #pragma unroll
-      for (int g = 0; g < kGroups; ++g) sum += s_cols[g * (G * kPerThread) + h];
-      dst[h] = sum;
+        for (int g = 0; g < kGroups; ++g) sum += s_dynamic[g * H + h];
+        dst[h] = sum;
+      }
     }
   };
   if (a.want_weight) emit(cw);
@@ -427,64 +538,82 @@ int sm_count() {
   return n;
 }
 
-int threads_per_row(int64_t H) { return H <= 32 * kPerThread ? 32 : H <= 128 * kPerThread ? 128 : 512; }
+// `width`: a row's values, and for shifted rows what a piece may stick out by
+int threads_per_row(int64_t width, int values) {
+  for (int G : {32, 64, 128, 256}) {
+    if (width <= G * values) return G;
+  }
+  return 1024;
+}
+enum { kSlack = 7 };           // values of a 16-byte piece that may lie before a shifted row
 
-// CTAs of a backward pass: two per SM, or as many as there are rows
-int64_t backward_ctas(int64_t rows, int64_t H) {
-  const int G = threads_per_row(H);
-  const int64_t per = threads_of(G) / G;
+// CTAs of a backward pass: three per SM (one of 1024 threads), or as many as there are rows; a multiple of eight row
+// groups, so that a thread's rows all start at the same place of a 16-byte piece
+int64_t backward_ctas(int64_t rows, int G) {
+  const int64_t per = threads_of(G) / G, unit = per >= 8 ? 1 : 8 / per;
   const int64_t need = (rows + per - 1) / per;
-  const int64_t most = 2 * static_cast<int64_t>(sm_count());
-  return need < most ? need : most;
+  const int64_t most = (G > 256 ? 1 : 3) * static_cast<int64_t>(sm_count()) / unit * unit;
+  return need < most ? (need + unit - 1) / unit * unit : most;
+}
+// of either way to see the rows: the workspace is sized before the pointers are known
+int64_t most_backward_ctas(int64_t rows, int64_t H) {
+  const int64_t a = backward_ctas(rows, threads_per_row(H, kBackward)), b = backward_ctas(rows, threads_per_row(H + kSlack, kBackward));
+  return a > b ? a : b;
 }
 
-template <typename T, typename P, int VEC, int G>
-void launch_fwd(const RowArgs& a, cudaStream_t s) {
+template <typename Kernel>
+int launch_rows(Kernel kernel, const RowArgs& a, int64_t grid, int threads, int smem, const char* what, cudaStream_t s) {
+  if (smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
+    return fail(GRMX_ERR_LAUNCH, "%s: cannot reserve %d bytes of shared memory: %s", what, smem, cudaGetErrorString(cudaGetLastError()));
+  }
+  kernel<<<static_cast<unsigned>(grid), threads, smem, s>>>(a);
+  return check_launch(what);
+}
+
+template <typename T, int VEC, int G, int ACCESS>
+int launch_group(const RowArgs& a, bool backward, cudaStream_t s) {
   constexpr int kGroups = threads_of(G) / G;
-  const int64_t need = (a.rows + kGroups - 1) / kGroups;
-  const unsigned grid = static_cast<unsigned>(need < 0x7fffffffLL ? need : 0x7fffffffLL);
-  if (a.gate != nullptr) fuse_norm_fwd_kernel<T, P, VEC, G, true><<<grid, threads_of(G), 0, s>>>(a);
-  else fuse_norm_fwd_kernel<T, P, VEC, G, false><<<grid, threads_of(G), 0, s>>>(a);
-}
-
-template <typename T, typename P, int VEC, int G>
-void launch_bwd(const RowArgs& a, cudaStream_t s) {
-  const unsigned grid = static_cast<unsigned>(backward_ctas(a.rows, a.H));
-  const int threads = threads_of(G);
-  if (a.gate != nullptr) {
-    if (a.scale != nullptr) fuse_norm_bwd_kernel<T, P, VEC, G, true, true><<<grid, threads, 0, s>>>(a);
-    else fuse_norm_bwd_kernel<T, P, VEC, G, true, false><<<grid, threads, 0, s>>>(a);
-  } else {
-    if (a.scale != nullptr) fuse_norm_bwd_kernel<T, P, VEC, G, false, true><<<grid, threads, 0, s>>>(a);
-    else fuse_norm_bwd_kernel<T, P, VEC, G, false, false><<<grid, threads, 0, s>>>(a);
-  }
-}
-
-template <typename T, typename P, int VEC>
-void launch_width(const RowArgs& a, bool backward, cudaStream_t s) {
-  const int G = threads_per_row(a.H);
   if (!backward) {
-    if (G == 32) launch_fwd<T, P, VEC, 32>(a, s);
-    else if (G == 128) launch_fwd<T, P, VEC, 128>(a, s);
-    else launch_fwd<T, P, VEC, 512>(a, s);
-  } else {
-    if (G == 32) launch_bwd<T, P, VEC, 32>(a, s);
-    else if (G == 128) launch_bwd<T, P, VEC, 128>(a, s);
-    else launch_bwd<T, P, VEC, 512>(a, s);
+    constexpr int64_t kUnit = kGroups >= 8 ? 1 : 8 / kGroups;
+    int64_t grid = ((a.rows + kGroups - 1) / kGroups + kUnit - 1) / kUnit * kUnit;
+    // shifted rows stage the parameters once per CTA: a CTA lives for several rows
+    const int64_t most = (ACCESS == kShifted ? 4 * static_cast<int64_t>(sm_count()) : 0x7ffffff0LL) / kUnit * kUnit;
+    if (grid > most) grid = most;
+    const int smem = ACCESS == kShifted ? 3 * staged_words(a.H) * 4 : 0;
+    return a.gate != nullptr ? launch_rows(fuse_norm_fwd_kernel<T, VEC, G, ACCESS, true>, a, grid, threads_of(G), smem, "fuse_norm", s)
+                             : launch_rows(fuse_norm_fwd_kernel<T, VEC, G, ACCESS, false>, a, grid, threads_of(G), smem, "fuse_norm", s);
+  }
+  const int64_t grid = backward_ctas(a.rows, G);
+  const int staged = ACCESS == kShifted ? 2 * staged_words(a.H) * 4 : 0, sums = kGroups > 1 ? kGroups * a.H * 4 : 0;
+  const int smem = staged > sums ? staged : sums;
+  const char* what = "fuse_norm gradient";
+  auto kernel = a.gate != nullptr ? (a.scale != nullptr ? fuse_norm_bwd_kernel<T, VEC, G, ACCESS, true, true> : fuse_norm_bwd_kernel<T, VEC, G, ACCESS, true, false>)
+                                  : (a.scale != nullptr ? fuse_norm_bwd_kernel<T, VEC, G, ACCESS, false, true> : fuse_norm_bwd_kernel<T, VEC, G, ACCESS, false, false>);
+  return launch_rows(kernel, a, grid, threads_of(G), smem, what, s);
+}
+
+template <typename T, int VEC, int ACCESS>
+int launch_width(const RowArgs& a, bool backward, cudaStream_t s) {
+  switch (threads_per_row(a.H + (ACCESS == kShifted ? kSlack : 0), backward ? kBackward : kForward)) {
+    case 32: return launch_group<T, VEC, 32, ACCESS>(a, backward, s);
+    case 64: return launch_group<T, VEC, 64, ACCESS>(a, backward, s);
+    case 128: return launch_group<T, VEC, 128, ACCESS>(a, backward, s);
+    case 256: return launch_group<T, VEC, 256, ACCESS>(a, backward, s);
+    default: return launch_group<T, VEC, 1024, ACCESS>(a, backward, s);
   }
 }
 
-void launch_types(const RowArgs& a, int dtype, int param_dtype, bool vec, bool backward, cudaStream_t s) {
-  if (dtype == GRMX_F32) {
-    if (vec) launch_width<float, float, 4>(a, backward, s);
-    else launch_width<float, float, 1>(a, backward, s);
-  } else if (param_dtype == GRMX_F32) {
-    if (vec) launch_width<__nv_bfloat16, float, 8>(a, backward, s);
-    else launch_width<__nv_bfloat16, float, 1>(a, backward, s);
-  } else {
-    if (vec) launch_width<__nv_bfloat16, __nv_bfloat16, 8>(a, backward, s);
-    else launch_width<__nv_bfloat16, __nv_bfloat16, 1>(a, backward, s);
-  }
+template <typename T>
+int launch_access(const RowArgs& a, int access, bool backward, cudaStream_t s) {
+  constexpr int kVec = 16 / static_cast<int>(sizeof(T));
+  if (access == kWhole) return launch_width<T, kVec, kWhole>(a, backward, s);
+  if (access == kShifted) return launch_width<T, kVec, kShifted>(a, backward, s);
+  return launch_width<T, 1, kSingle>(a, backward, s);
+}
+
+int launch_types(RowArgs& a, int dtype, int param_dtype, int access, bool backward, cudaStream_t s) {
+  a.param_bf16 = param_dtype == GRMX_BF16;
+  return dtype == GRMX_F32 ? launch_access<float>(a, access, backward, s) : launch_access<__nv_bfloat16>(a, access, backward, s);
 }
 
 int check_common(const char* who, int64_t rows, int64_t H, int dtype, int param_dtype) {
@@ -495,11 +624,14 @@ int check_common(const char* who, int64_t rows, int64_t H, int dtype, int param_
   return GRMX_OK;
 }
 
-// 16-byte pieces where every row and every parameter starts on a 16-byte boundary
-bool whole_pieces(int64_t H, int dtype, const void* const* ptrs, int n) {
-  uintptr_t all = 0;
-  for (int i = 0; i < n; ++i) all |= reinterpret_cast<uintptr_t>(ptrs[i]);
-  return (all & 15u) == 0 && H % (dtype == GRMX_F32 ? 4 : 8) == 0;
+// 16-byte pieces where every tensor starts on a 16-byte boundary, shifted where the rows do not
+int access_of(int64_t H, int dtype, const void* const* rows, int n_rows, const void* const* params, int n_params) {
+  uintptr_t row_bits = 0, param_bits = 0;
+  for (int i = 0; i < n_rows; ++i) row_bits |= reinterpret_cast<uintptr_t>(rows[i]);
+  for (int i = 0; i < n_params; ++i) param_bits |= reinterpret_cast<uintptr_t>(params[i]);
+  if ((row_bits & 15u) != 0) return kSingle;
+  if (H % (dtype == GRMX_F32 ? 4 : 8) == 0 && (param_bits & 15u) == 0) return kWhole;
+  return H + kSlack <= kMaxWidth ? kShifted : kSingle;
 }
 
 }  // namespace
@@ -527,15 +659,15 @@ extern "C" int grmx_fuse_norm_fwd(const void* online, const void* update, const 
   a.stats = reinterpret_cast<float2*>(row_stats);
   a.rows = rows;
   a.H = static_cast<int>(H);
-  const void* ptrs[] = {online, update, gate, scale, ln_weight, ln_bias, out, sum_out};
-  launch_types(a, dtype, param_dtype, whole_pieces(H, dtype, ptrs, 8), false, static_cast<cudaStream_t>(stream));
-  return check_launch("fuse_norm");
+  const void* row_ptrs[] = {online, update, gate, out, sum_out};
+  const void* param_ptrs[] = {scale, ln_weight, ln_bias};
+  return launch_types(a, dtype, param_dtype, access_of(H, dtype, row_ptrs, 5, param_ptrs, 3), false, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int64_t grmx_fuse_norm_workspace(int64_t rows, int64_t H) {
   using namespace grmx;
   if (check_common("grmx_fuse_norm_workspace", rows, H, GRMX_F32, GRMX_F32) != GRMX_OK) return -1;
-  return rows == 0 ? 0 : 3 * backward_ctas(rows, H) * H * 4;
+  return rows == 0 ? 0 : 3 * most_backward_ctas(rows, H) * H * 4;
 }
 
 extern "C" int grmx_fuse_norm_bwd(const void* grad_out, const void* grad_sum, const void* online, const void* update,
@@ -579,16 +711,17 @@ extern "C" int grmx_fuse_norm_bwd(const void* grad_out, const void* grad_sum, co
   a.want_scale = grad_scale != nullptr;
   a.want_weight = grad_weight != nullptr;
   a.want_bias = grad_bias != nullptr;
-  const int64_t ctas = backward_ctas(rows, H);
+  const void* row_ptrs[] = {online, update, gate, grad_out, grad_sum, grad_online, grad_update, grad_gate};
+  const void* param_ptrs[] = {scale, ln_weight};
+  const int access = access_of(H, dtype, row_ptrs, 8, param_ptrs, 2);
+  const int64_t ctas = backward_ctas(rows, threads_per_row(H + (access == kShifted ? kSlack : 0), kBackward));
   if (kinds > 0) {
-    GRMX_REQUIRE(workspace != nullptr && workspace_bytes >= 3 * ctas * H * 4, "%s: workspace of %lld bytes, needs %lld", who,
-                 (long long)workspace_bytes, (long long)(3 * ctas * H * 4));
+    GRMX_REQUIRE(workspace != nullptr && workspace_bytes >= 3 * most_backward_ctas(rows, H) * H * 4, "%s: workspace of %lld bytes, needs %lld", who,
+                 (long long)workspace_bytes, (long long)(3 * most_backward_ctas(rows, H) * H * 4));
     GRMX_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15u) == 0, "%s: workspace must be 16-byte aligned", who);
     a.col_partials = static_cast<float*>(workspace);
   }
-  const void* ptrs[] = {online, update, gate, scale, ln_weight, grad_out, grad_sum, grad_online, grad_update, grad_gate};
-  launch_types(a, dtype, param_dtype, whole_pieces(H, dtype, ptrs, 10), true, s);
-  int status = check_launch("fuse_norm gradient");
+  const int status = launch_types(a, dtype, param_dtype, access, true, s);
   if (status != GRMX_OK || kinds == 0) return status;
   void* outs[3] = {nullptr, nullptr, nullptr};
   int n = 0;
