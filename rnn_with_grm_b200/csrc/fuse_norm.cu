@@ -505,24 +505,28 @@ fuse_norm_bwd_kernel(const __grid_constant__ RowArgs a) {
   }
 }
 
-// out_k[h] = sum over the CTAs' partials, in order: 32 columns x 8 slices per block
+// out_k[h] = sum over the CTAs' partials, in order: 32 columns x 32 slices per block
 template <typename P>
-__global__ void __launch_bounds__(256) fuse_norm_cols_kernel(const float* __restrict__ partials, int ctas, int H, P* out0, P* out1,
-                                                             P* out2) {
-  __shared__ float s_sum[8][32];
+__global__ void __launch_bounds__(1024) fuse_norm_cols_kernel(const float* __restrict__ partials, int ctas, int H, P* out0, P* out1,
+                                                              P* out2) {
+  __shared__ float s_sum[32][33];
   const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
   const int h = blockIdx.x * 32 + lane;
   const float* src = partials + static_cast<int64_t>(blockIdx.y) * ctas * H;
   float sum = 0.0f;
   if (h < H) {
-    for (int i = slice; i < ctas; i += 8) sum += src[static_cast<int64_t>(i) * H + h];
+#pragma unroll 4
+    for (int i = slice; i < ctas; i += 32) sum += src[static_cast<int64_t>(i) * H + h];
   }
   s_sum[slice][lane] = sum;
   __syncthreads();
-  if (slice == 0 && h < H) {
-    for (int i = 1; i < 8; ++i) sum += s_sum[i][lane];
+  sum = s_sum[lane][slice];            // column `slice` of the block, one slice per lane
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  const int col = blockIdx.x * 32 + slice;
+  if (lane == 0 && col < H) {
     P* out = blockIdx.y == 0 ? out0 : blockIdx.y == 1 ? out1 : out2;
-    out[h] = from_float<P>(sum);
+    out[col] = from_float<P>(sum);
   }
 }
 
@@ -730,10 +734,10 @@ extern "C" int grmx_fuse_norm_bwd(const void* grad_out, const void* grad_sum, co
   }
   const dim3 grid(static_cast<unsigned>((H + 31) / 32), static_cast<unsigned>(kinds));
   if (param_dtype == GRMX_F32) {
-    fuse_norm_cols_kernel<float><<<grid, 256, 0, s>>>(a.col_partials, static_cast<int>(ctas), a.H, static_cast<float*>(outs[0]),
+    fuse_norm_cols_kernel<float><<<grid, 1024, 0, s>>>(a.col_partials, static_cast<int>(ctas), a.H, static_cast<float*>(outs[0]),
                                                        static_cast<float*>(outs[1]), static_cast<float*>(outs[2]));
   } else {
-    fuse_norm_cols_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(
+    fuse_norm_cols_kernel<__nv_bfloat16><<<grid, 1024, 0, s>>>(
         a.col_partials, static_cast<int>(ctas), a.H, static_cast<__nv_bfloat16*>(outs[0]), static_cast<__nv_bfloat16*>(outs[1]),
         static_cast<__nv_bfloat16*>(outs[2]));
   }

@@ -9,6 +9,9 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <torch/csrc/autograd/functions/basic_ops.h>
+
+#include <array>
 #include <atomic>
 #include <cmath>
 #include <tuple>
@@ -549,7 +552,7 @@ at::Tensor retrieve_fuse_tc_cuda(const at::Tensor& archive, const at::Tensor& in
   return out;
 }
 
-// ---- vocabulary loss: hidden [N,D] and weight [V,D] (bf16 or fp32), targets int64 [N], bias [V]? ----
+// ---- vocabulary loss: hidden [...,D] and weight [V,D] (bf16 or fp32), targets int64 [...], bias [V]? ----
 
 struct LossArgs {
   at::Tensor hidden, weight, targets, bias;
@@ -559,10 +562,10 @@ struct LossArgs {
 
 LossArgs check_loss_inputs(const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& targets,
                            const c10::optional<at::Tensor>& bias, int64_t reduction) {
-  TORCH_CHECK(hidden.dim() == 2, "hidden must have shape [N, D]");
+  TORCH_CHECK(hidden.dim() >= 1, "hidden must have shape [..., D]");
   TORCH_CHECK(weight.dim() == 2, "weight must have shape [V, D]");
-  TORCH_CHECK(hidden.size(1) == weight.size(1), "feature dim mismatch between hidden and weight");
-  TORCH_CHECK(targets.dim() == 1 && targets.size(0) == hidden.size(0), "targets must have shape [N]");
+  TORCH_CHECK(hidden.size(-1) == weight.size(1), "feature dim mismatch between hidden and weight");
+  TORCH_CHECK(targets.sizes() == hidden.sizes().slice(0, hidden.dim() - 1), "targets must have the shape of hidden without its features");
   TORCH_CHECK(weight.size(0) > 0 && weight.size(1) > 0, "weight must not be empty");
   require_cuda(hidden, "hidden");
   require_cuda(weight, "weight");
@@ -578,8 +581,8 @@ LossArgs check_loss_inputs(const at::Tensor& hidden, const at::Tensor& weight, c
   a.hidden = hidden.contiguous();
   a.weight = weight.contiguous();
   a.targets = targets.to(at::kLong).contiguous();
-  a.N = hidden.size(0);
-  a.D = hidden.size(1);
+  a.N = targets.numel();
+  a.D = weight.size(1);
   a.V = weight.size(0);
   a.dtype = a.bias_dtype = dtype_code(hidden.scalar_type(), "hidden");
   if (bias.has_value() && bias->defined()) {
@@ -607,7 +610,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_xent_fwd_cuda(const at::Te
   LossArgs a = check_loss_inputs(hidden, weight, targets, bias, reduction);
   c10::cuda::CUDAGuard guard(a.hidden.device());
   const auto f32 = a.hidden.options().dtype(at::kFloat);
-  auto loss = reduction == GRMX_REDUCE_NONE ? at::empty({a.N}, f32) : at::empty({}, f32);
+  auto loss = reduction == GRMX_REDUCE_NONE ? at::empty(targets.sizes(), f32) : at::empty({}, f32);
   auto stats = at::empty({2, a.N}, f32);
   auto inv_count = at::empty({1}, f32);
   if (a.N == 0) {      // no token: an empty list, a sum of 0, a mean of 0 / 0
@@ -734,8 +737,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tenso
     const c10::optional<at::Tensor>& grad_out, const c10::optional<at::Tensor>& grad_sum, const at::Tensor& online,
     const at::Tensor& update, const c10::optional<at::Tensor>& gate, const c10::optional<at::Tensor>& scale,
     const c10::optional<at::Tensor>& ln_weight, const c10::optional<at::Tensor>& ln_bias, const at::Tensor& row_stats,
-    c10::List<bool> want) {
-  TORCH_CHECK(want.size() == 6, "want must name six gradients");
+    std::array<bool, 6> want) {
   FuseNormArgs a = check_fuse_norm_inputs(online, update, gate, scale, ln_weight, ln_bias);
   TORCH_CHECK(row_stats.is_cuda() && row_stats.device() == a.online.device() && row_stats.scalar_type() == at::kFloat &&
                   row_stats.is_contiguous() && row_stats.numel() == 2 * a.rows,
@@ -767,6 +769,119 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tenso
                                   ptr_or_null(d_gate), ptr_or_null(d_scale), ptr_or_null(d_weight), ptr_or_null(d_bias),
                                   a.rows, a.H, a.dtype, a.param_dtype, ptr_or_null(ws), ws.numel(), current_stream()));
   return {d_online, d_update, d_gate, d_scale, d_weight, d_bias};
+}
+
+// ---- the same with autograd: in C++, so that a training step spends its host time on launches ----
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+c10::optional<at::Tensor> maybe(const at::Tensor& t) { return t.defined() ? c10::optional<at::Tensor>(t) : c10::nullopt; }
+at::Tensor or_undefined(const c10::optional<at::Tensor>& t) { return t.has_value() ? *t : at::Tensor(); }
+at::Tensor if_wanted(const at::Tensor& t, bool wanted) { return wanted ? t : at::Tensor(); }
+using MaybeTensor = c10::optional<at::Tensor>;
+
+// gradients with a gradient of their own are asked for (create_graph): they get one that reports its absence
+variable_list no_second_derivative(variable_list grads, const char* what) {
+  if (!at::GradMode::is_enabled()) return grads;
+  std::vector<size_t> at_index;
+  variable_list defined;
+  for (size_t i = 0; i < grads.size(); ++i) {
+    if (grads[i].defined()) {
+      at_index.push_back(i);
+      defined.push_back(grads[i].requires_grad() ? grads[i] : grads[i].detach().requires_grad_());
+    }
+  }
+  auto node = std::make_shared<torch::autograd::DelayedError>(std::string(what) + " is differentiable once only",
+                                                              static_cast<int64_t>(defined.size()));
+  variable_list marked = (*node)(std::move(defined));
+  for (size_t i = 0; i < at_index.size(); ++i) grads[at_index[i]] = marked[i];
+  return grads;
+}
+
+struct LinearCrossEntropyFn : public torch::autograd::Function<LinearCrossEntropyFn> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& hidden, const at::Tensor& weight, const MaybeTensor& bias,
+                            const at::Tensor& targets, int64_t ignore_index, int64_t reduction) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [loss, stats, inv_count] = linear_xent_fwd_cuda(hidden, weight, targets, bias, ignore_index, reduction);
+    ctx->save_for_backward({hidden, weight, or_undefined(bias), targets, stats, inv_count});
+    ctx->saved_data["ignore_index"] = ignore_index;
+    ctx->saved_data["reduction"] = reduction;
+    return loss;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const bool wh = ctx->needs_input_grad(0), ww = ctx->needs_input_grad(1), wb = saved[2].defined() && ctx->needs_input_grad(2);
+    variable_list out(6);
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      auto [dh, dw, db] = linear_xent_bwd_cuda(grads[0], saved[0], saved[1], saved[3], maybe(saved[2]), saved[4], saved[5],
+                                               ctx->saved_data["ignore_index"].toInt(), ctx->saved_data["reduction"].toInt(), wh, ww, wb);
+      out[0] = if_wanted(dh, wh);
+      out[1] = if_wanted(dw, ww);
+      out[2] = if_wanted(db, wb);
+    }
+    return no_second_derivative(std::move(out), "linear_cross_entropy");
+  }
+};
+
+at::Tensor linear_cross_entropy(const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& targets,
+                                const c10::optional<at::Tensor>& bias, int64_t ignore_index, int64_t reduction) {
+  const at::Tensor b = or_undefined(bias);
+  if (at::GradMode::is_enabled() && (hidden.requires_grad() || weight.requires_grad() || (b.defined() && b.requires_grad()))) {
+    return LinearCrossEntropyFn::apply(hidden, weight, maybe(b), targets, ignore_index, reduction);
+  }
+  at::AutoDispatchBelowADInplaceOrView below;
+  return std::get<0>(linear_xent_fwd_cuda(hidden, weight, targets, bias, ignore_index, reduction));
+}
+
+struct FuseLayerNormFn : public torch::autograd::Function<FuseLayerNormFn> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& online, const at::Tensor& update, const MaybeTensor& gate,
+                               const MaybeTensor& scale, const MaybeTensor& weight, const MaybeTensor& bias, double eps, bool want_sum) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [out, sum, stats] = fuse_norm_fwd_cuda(online, update, gate, scale, weight, bias, eps, want_sum, true);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({online, update, or_undefined(gate), or_undefined(scale), or_undefined(weight), or_undefined(bias), stats});
+    return want_sum ? variable_list{out, sum} : variable_list{out};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list out(8);
+    const at::Tensor dy = grads[0], dsum = grads.size() > 1 ? grads[1] : at::Tensor();
+    if (!dy.defined() && !dsum.defined()) return out;
+    const auto saved = ctx->get_saved_variables();
+    bool want[6];
+    // inputs are numbered without the ones that were not given
+    for (size_t i = 0, given = 0; i < 6; ++i) want[i] = saved[i].defined() && ctx->needs_input_grad(given++);
+    // without gate and scale both row tensors have the same gradient: one is written
+    const bool shared = !saved[2].defined() && !saved[3].defined() && want[0] && want[1];
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      auto [d0, d1, d2, d3, d4, d5] = fuse_norm_bwd_cuda(maybe(dy), maybe(dsum), saved[0], saved[1], maybe(saved[2]), maybe(saved[3]),
+                                                         maybe(saved[4]), maybe(saved[5]), saved[6],
+                                                         {want[0], want[1] && !shared, want[2], want[3], want[4], want[5]});
+      out[0] = if_wanted(d0, want[0]);
+      out[1] = if_wanted(shared ? d0 : d1, want[1]);
+      out[2] = if_wanted(d2, want[2]);
+      out[3] = if_wanted(d3, want[3]);
+      out[4] = if_wanted(d4, want[4]);
+      out[5] = if_wanted(d5, want[5]);
+    }
+    return no_second_derivative(std::move(out), "fuse_layer_norm");
+  }
+};
+
+// (out,) or (out, sum)
+variable_list fuse_layer_norm(const at::Tensor& online, const at::Tensor& update, const c10::optional<at::Tensor>& weight,
+                              const c10::optional<at::Tensor>& bias, const c10::optional<at::Tensor>& gate,
+                              const c10::optional<at::Tensor>& scale, double eps, bool want_sum) {
+  const at::Tensor g = or_undefined(gate), k = or_undefined(scale), w = or_undefined(weight), b = or_undefined(bias);
+  auto needs = [](const at::Tensor& t) { return t.defined() && t.requires_grad(); };
+  if (at::GradMode::is_enabled() && (needs(online) || needs(update) || needs(g) || needs(k) || needs(w) || needs(b))) {
+    return FuseLayerNormFn::apply(online, update, maybe(g), maybe(k), maybe(w), maybe(b), eps, want_sum);
+  }
+  at::AutoDispatchBelowADInplaceOrView below;
+  auto [out, sum, stats] = fuse_norm_fwd_cuda(online, update, gate, scale, weight, bias, eps, want_sum, false);
+  return want_sum ? variable_list{out, sum} : variable_list{out};
 }
 
 }  // namespace
@@ -801,7 +916,7 @@ TORCH_LIBRARY(grmx, m) {
   m.def("linear_xent_fwd(Tensor hidden, Tensor weight, Tensor targets, Tensor? bias, int ignore_index, int reduction) -> (Tensor loss, Tensor row_stats, Tensor inv_count)");
   m.def("linear_xent_bwd(Tensor grad_loss, Tensor hidden, Tensor weight, Tensor targets, Tensor? bias, Tensor row_stats, Tensor inv_count, int ignore_index, int reduction, bool want_hidden, bool want_weight, bool want_bias) -> (Tensor grad_hidden, Tensor grad_weight, Tensor grad_bias)");
   m.def("fuse_norm_fwd(Tensor online, Tensor update, Tensor? gate, Tensor? scale, Tensor? ln_weight, Tensor? ln_bias, float eps, bool want_sum, bool want_stats) -> (Tensor out, Tensor sum, Tensor row_stats)");
-  m.def("fuse_norm_bwd(Tensor? grad_out, Tensor? grad_sum, Tensor online, Tensor update, Tensor? gate, Tensor? scale, Tensor? ln_weight, Tensor? ln_bias, Tensor row_stats, bool[] want) -> (Tensor grad_online, Tensor grad_update, Tensor grad_gate, Tensor grad_scale, Tensor grad_weight, Tensor grad_bias)");
+  m.def("fuse_norm_bwd(Tensor? grad_out, Tensor? grad_sum, Tensor online, Tensor update, Tensor? gate, Tensor? scale, Tensor? ln_weight, Tensor? ln_bias, Tensor row_stats, bool[6] want) -> (Tensor grad_online, Tensor grad_update, Tensor grad_gate, Tensor grad_scale, Tensor grad_weight, Tensor grad_bias)");
   m.def("select_fuse(Tensor states, Tensor indices, Tensor gates, Tensor? online, Tensor? ln_weight, Tensor? ln_bias, float ln_eps, int mode) -> Tensor");
 }
 
@@ -841,5 +956,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     check_status(grmx_device_error_word(&word, current_stream()));
     return word;
   });
+  // the training operators with autograd (Python: loss.linear_cross_entropy, fusion.fuse_layer_norm)
+  m.def("linear_cross_entropy", linear_cross_entropy, pybind11::call_guard<pybind11::gil_scoped_release>());
+  m.def("fuse_layer_norm", fuse_layer_norm, pybind11::call_guard<pybind11::gil_scoped_release>());
   m.def("device_error_reset", []() { check_status(grmx_device_error_reset(current_stream())); });
 }

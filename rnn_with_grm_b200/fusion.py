@@ -14,41 +14,8 @@ from typing import Optional, Tuple, Union
 
 import torch
 from torch import Tensor
-from torch.autograd.function import once_differentiable
 
 from . import cuda_ops
-
-
-class FuseLayerNormFn(torch.autograd.Function):
-    """``(online, update, gate?, scale?, weight?, bias?) -> (out, sum)``; ``sum`` is empty unless asked for."""
-
-    @staticmethod
-    def forward(ctx, online: Tensor, update: Tensor, gate: Optional[Tensor], scale: Optional[Tensor],
-                weight: Optional[Tensor], bias: Optional[Tensor], eps: float, want_sum: bool):
-        out, total, row_stats = torch.ops.grmx.fuse_norm_fwd(online, update, gate, scale, weight, bias, eps, want_sum, True)
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(online, update, gate, scale, weight, bias, row_stats)
-        ctx.want_sum = want_sum
-        if not want_sum:
-            ctx.mark_non_differentiable(total)
-        return out, total
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_out: Optional[Tensor], grad_sum: Optional[Tensor]):
-        grad_sum = grad_sum if ctx.want_sum else None
-        if grad_out is None and grad_sum is None:
-            return (None,) * 8
-        online, update, gate, scale, weight, bias, row_stats = ctx.saved_tensors
-        want = list(ctx.needs_input_grad[:6])
-        # without gate and scale both row tensors have the same gradient: one is written
-        shared = gate is None and scale is None and want[0] and want[1]
-        asked = want if not shared else [True, False, *want[2:]]
-        grads = torch.ops.grmx.fuse_norm_bwd(grad_out, grad_sum, online, update, gate, scale, weight, bias, row_stats, asked)
-        grads = [grad if wanted else None for grad, wanted in zip(grads, asked)]
-        if shared:
-            grads[1] = grads[0]
-        return (*grads, None, None)
 
 
 def fuse_layer_norm(online: Tensor, update: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, *,
@@ -65,11 +32,7 @@ def fuse_layer_norm(online: Tensor, update: Tensor, weight: Optional[Tensor] = N
     cuda_ops._require_extension("fuse_layer_norm")
     if online.device.type != "cuda":
         raise RuntimeError(f"fuse_layer_norm: tensors must be on a CUDA device, got {online.device}; this engine has no CPU path.")
-    leaves = (online, update, gate, scale, weight, bias)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in leaves):
-        out, total = FuseLayerNormFn.apply(online, update, gate, scale, weight, bias, float(eps), bool(return_sum))
-    else:
-        out, total, _ = torch.ops.grmx.fuse_norm_fwd(online, update, gate, scale, weight, bias, float(eps), bool(return_sum), False)
+    out = cuda_ops._Extension.module.fuse_layer_norm(online, update, weight, bias, gate, scale, float(eps), bool(return_sum))
     if cuda_ops._checking_each_call() and not torch.cuda.is_current_stream_capturing():
         cuda_ops.check_device_errors()
-    return (out, total) if return_sum else out
+    return (out[0], out[1]) if return_sum else out[0]

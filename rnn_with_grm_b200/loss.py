@@ -13,33 +13,10 @@ from typing import Optional
 
 import torch
 from torch import Tensor
-from torch.autograd.function import once_differentiable
 
 from . import cuda_ops
 
 _REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
-
-
-class LinearCrossEntropyFn(torch.autograd.Function):
-    """``hidden [N, D], weight [V, D], targets [N], bias [V]?`` -> loss ``[N]`` or scalar, float32."""
-
-    @staticmethod
-    def forward(ctx, hidden: Tensor, weight: Tensor, targets: Tensor, bias: Optional[Tensor], ignore_index: int,
-                reduction: int):
-        loss, row_stats, inv_count = torch.ops.grmx.linear_xent_fwd(hidden, weight, targets, bias, ignore_index, reduction)
-        ctx.save_for_backward(hidden, weight, targets, bias, row_stats, inv_count)
-        ctx.ignore_index, ctx.reduction = ignore_index, reduction
-        return loss
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_loss: Tensor):
-        hidden, weight, targets, bias, row_stats, inv_count = ctx.saved_tensors
-        want = (ctx.needs_input_grad[0], ctx.needs_input_grad[1], ctx.needs_input_grad[3])
-        grads = torch.ops.grmx.linear_xent_bwd(grad_loss, hidden, weight, targets, bias, row_stats, inv_count,
-                                               ctx.ignore_index, ctx.reduction, *want)
-        d_hidden, d_weight, d_bias = (grad if wanted else None for grad, wanted in zip(grads, want))
-        return d_hidden, d_weight, None, d_bias, None, None
 
 
 def linear_cross_entropy(hidden: Tensor, weight: Tensor, targets: Tensor, bias: Optional[Tensor] = None, *,
@@ -63,12 +40,7 @@ def linear_cross_entropy(hidden: Tensor, weight: Tensor, targets: Tensor, bias: 
         raise ValueError(f"hidden [..., D] and weight [V, D] do not fit: {tuple(hidden.shape)}, {tuple(weight.shape)}")
     if targets.shape != hidden.shape[:-1]:
         raise ValueError(f"targets must have the shape {tuple(hidden.shape[:-1])}, got {tuple(targets.shape)}")
-    rows, flat = hidden.reshape(-1, hidden.shape[-1]), targets.reshape(-1)
-    code = _REDUCTIONS[reduction]
-    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
-        loss = LinearCrossEntropyFn.apply(rows, weight, flat, bias, int(ignore_index), code)
-    else:
-        loss = torch.ops.grmx.linear_xent_fwd(rows, weight, flat, bias, int(ignore_index), code)[0]
+    loss = cuda_ops._Extension.module.linear_cross_entropy(hidden, weight, targets, bias, int(ignore_index), _REDUCTIONS[reduction])
     if cuda_ops._checking_each_call() and not torch.cuda.is_current_stream_capturing():
         cuda_ops.check_device_errors()
-    return loss.reshape(targets.shape) if reduction == "none" else loss
+    return loss
