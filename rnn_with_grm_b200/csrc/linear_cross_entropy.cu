@@ -101,47 +101,237 @@ int make_operand(Operand* out, const void* src, int64_t rows, int64_t cols, int 
   return check_launch("loss operand planes");
 }
 
+// ------------------------------------------------------------------ a few tokens
+
+// two (maximum, sum of 2^(score - maximum)) pairs into one
+__device__ __forceinline__ float2 join(float2 a, float2 b) {
+  const float next = fmaxf(a.x, b.x);
+  const float base = next == -INFINITY ? 0.0f : next;       // neither has a finite score
+  return make_float2(next, a.y * exp2_fast(a.x - base) + b.y * exp2_fast(b.x - base));
+}
+
+// Up to eight tokens (a decoding step): bound by the stream of W, one pass over it with plain fused multiply-adds.
+// A warp takes ROWS words at a time, a lane 32 bytes of each; the tokens' features wait in shared memory.  The lanes' sums are exchanged so that every lane ends up with the score of one (word, token) and
+// keeps that pair's running maximum and sum; lanes, warps and (in loss_join_kernel) CTAs are joined at the end.
+// One token, 512 x 32768 bf16: 21 us as a padded tile of the product, 11.5 us so (2.9 TB/s, half of it latency).
+constexpr int kFewTokens = 8;
+constexpr int kFewThreads = 256;
+
+// sum of each of M values over the lanes; lane l returns that of value l / (32 / M)
+template <int M>
+__device__ __forceinline__ float spread_sums(float (&v)[M], int lane) {
+  int width = M;
+#pragma unroll
+  for (int half = 16; half >= 1; half >>= 1) {
+    if (width > 1) {
+      const bool upper = (lane & half) != 0;
+      width >>= 1;
+#pragma unroll
+      for (int j = 0; j < M / 2; ++j) {
+        if (j < width) {
+          const float keep = upper ? v[j + width] : v[j];
+          const float give = upper ? v[j] : v[j + width];
+          v[j] = keep + __shfl_xor_sync(0xffffffffu, give, half);
+        }
+      }
+    } else {
+      v[0] += __shfl_xor_sync(0xffffffffu, v[0], half);
+    }
+  }
+  return v[0];
+}
+
+// 16 bytes of features: whole where they are all there, value by value at a row's end or off a 16-byte boundary
+template <typename T>
+__device__ __forceinline__ uint4 load_features(const T* row, int d, int D, bool aligned) {
+  constexpr int G = 16 / sizeof(T);
+  if (aligned && d + G <= D) return __ldcs(reinterpret_cast<const uint4*>(row + d));
+  union { T v[G]; uint4 q; } u;
+#pragma unroll
+  for (int e = 0; e < G; ++e) u.v[e] = d + e < D ? row[d + e] : from_float<T>(0.0f);
+  return u.q;
+}
+template <typename T>
+__device__ __forceinline__ void widen(uint4 q, float (&x)[16 / sizeof(T)]) {
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if constexpr (sizeof(T) == 2) {
+      x[2 * e] = __uint_as_float(w[e] << 16);
+      x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+    } else {
+      x[e] = __uint_as_float(w[e]);
+    }
+  }
+}
+
+template <typename T, int TOKENS, int ROWS>
+__global__ void __launch_bounds__(kFewThreads)
+few_tokens_kernel(const T* __restrict__ hidden, const T* __restrict__ weight, const void* __restrict__ bias, int bias_dtype,
+                  const int64_t* __restrict__ targets, int64_t ignore_index, int tokens, int D, int64_t V, int aligned,
+                  float2* __restrict__ partials, float* __restrict__ target_score, uint32_t* ticket) {
+  constexpr int G = 16 / static_cast<int>(sizeof(T)), kChunk = 64 * G;       // features per piece, and per chunk of two pieces
+  constexpr int M = TOKENS * ROWS, kLanesPer = 32 / M;
+  static_assert(M <= 32, "a lane holds one (word, token)");
+  extern __shared__ float s_x[];                           // [TOKENS][D rounded up to whole chunks], zero beyond D
+  __shared__ float2 s_part[kFewThreads / 32][TOKENS];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int pitch = (D + kChunk - 1) / kChunk * kChunk;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * (kFewThreads / 32) * ROWS;
+  int64_t v0 = (static_cast<int64_t>(blockIdx.x) * (kFewThreads / 32) + warp) * ROWS;
+  uint4 raw[ROWS][2];
+  auto load = [&](int64_t first, int d0) {
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      const T* row = weight + (first + r < V ? first + r : V - 1) * D;       // words beyond the last are not counted below
+#pragma unroll
+      for (int h = 0; h < 2; ++h) raw[r][h] = load_features(row, d0 + (h * 32 + lane) * G, D, aligned != 0);
+    }
+  };
+  load(v0, 0);                                             // on its way while the tokens are staged
+  if (blockIdx.x == 0 && threadIdx.x == 0) *ticket = 0u;
+  for (int i = threadIdx.x; i < TOKENS * pitch; i += kFewThreads) {
+    const int t = i / pitch, d = i - t * pitch;
+    s_x[i] = t < tokens && d < D ? to_float<T>(hidden[static_cast<int64_t>(t) * D + d]) : 0.0f;
+  }
+  const int mine = lane / kLanesPer, my_row = mine / TOKENS, my_token = mine % TOKENS;
+  int64_t my_target = -1;
+  if (my_token < tokens) {
+    const int64_t t = targets[my_token];
+    if (t != ignore_index) my_target = t;
+  }
+  __syncthreads();
+  float2 all = make_float2(-INFINITY, 0.0f);
+  for (bool loaded = true; v0 < V; v0 += step) {
+    const int64_t v = v0 + my_row;
+    float b = 0.0f;
+    if (bias != nullptr && v < V) {
+      b = bias_dtype == GRMX_F32 ? static_cast<const float*>(bias)[v] : __bfloat162float(static_cast<const __nv_bfloat16*>(bias)[v]);
+    }
+    float acc[M];
+#pragma unroll
+    for (int i = 0; i < M; ++i) acc[i] = 0.0f;
+    for (int d0 = 0; d0 < D; d0 += kChunk) {
+      if (!loaded) load(v0, d0);
+      loaded = false;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float w[ROWS][G];
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) widen<T>(raw[r][h], w[r]);
+#pragma unroll
+        for (int t = 0; t < TOKENS; ++t) {
+#pragma unroll
+          for (int e = 0; e < G; e += 4) {
+            const float4 x = *reinterpret_cast<const float4*>(s_x + t * pitch + d0 + (h * 32 + lane) * G + e);
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) {
+              float& a = acc[r * TOKENS + t];
+              a = fmaf(x.x, w[r][e], a);
+              a = fmaf(x.y, w[r][e + 1], a);
+              a = fmaf(x.z, w[r][e + 2], a);
+              a = fmaf(x.w, w[r][e + 3], a);
+            }
+          }
+        }
+      }
+    }
+    const float y = fmaf(spread_sums<M>(acc, lane), kLog2e, b * kLog2e);
+    if (v < V) {
+      if (v == my_target && lane % kLanesPer == 0) target_score[my_token] = y;
+      const float next = fmaxf(all.x, y);
+      const float base = next == -INFINITY ? 0.0f : next;
+      all = make_float2(next, fmaf(all.y, exp2_fast(all.x - base), exp2_fast(y - base)));
+    }
+  }
+  // lanes with the same token (other words), then warps
+#pragma unroll
+  for (int o = kLanesPer * TOKENS; o < 32; o <<= 1) {
+    all = join(all, make_float2(__shfl_xor_sync(0xffffffffu, all.x, o), __shfl_xor_sync(0xffffffffu, all.y, o)));
+  }
+  if (my_row == 0 && lane % kLanesPer == 0) s_part[warp][my_token] = all;
+  __syncthreads();
+  if (threadIdx.x < tokens) {
+    float2 sum = s_part[0][threadIdx.x];
+    for (int i = 1; i < kFewThreads / 32; ++i) sum = join(sum, s_part[i][threadIdx.x]);
+    partials[static_cast<int64_t>(blockIdx.x) * tokens + threadIdx.x] = sum;
+  }
+}
+
+constexpr int kFewRows = 8;                                // words at a time per warp (4 with eight tokens)
+int few_tokens_blocks(int64_t V) {
+  const int64_t need = (V + kFewThreads / 32 * kFewRows - 1) / (kFewThreads / 32 * kFewRows);
+  return static_cast<int>(need < 4 * 148 ? need : 4 * 148);
+}
+
+template <typename T>
+int launch_few_tokens(const void* hidden, const void* weight, const void* bias, int bias_dtype, const int64_t* targets,
+                      int64_t ignore_index, int tokens, int D, int64_t V, float2* partials, float* target_score,
+                      uint32_t* ticket, cudaStream_t s) {
+  constexpr int kChunk = 1024 / static_cast<int>(sizeof(T));
+  const int padded = tokens <= 1 ? 1 : tokens <= 2 ? 2 : tokens <= 4 ? 4 : 8;
+  const int smem = padded * ((D + kChunk - 1) / kChunk * kChunk) * 4;
+  const int aligned = D % (16 / static_cast<int>(sizeof(T))) == 0 && (reinterpret_cast<uintptr_t>(weight) & 15u) == 0;
+  auto kernel = padded == 1   ? few_tokens_kernel<T, 1, kFewRows>
+                : padded == 2 ? few_tokens_kernel<T, 2, kFewRows>
+                : padded == 4 ? few_tokens_kernel<T, 4, kFewRows>
+                              : few_tokens_kernel<T, 8, 4>;
+  if (smem > 40 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
+    return fail(GRMX_ERR_LAUNCH, "loss of a few tokens: cannot reserve %d bytes of shared memory: %s", smem, cudaGetErrorString(cudaGetLastError()));
+  }
+  kernel<<<few_tokens_blocks(V), kFewThreads, smem, s>>>(static_cast<const T*>(hidden), static_cast<const T*>(weight), bias, bias_dtype,
+                                                         targets, ignore_index, tokens, D, V, aligned, partials, target_score, ticket);
+  return check_launch("loss of a few tokens");
+}
+
+// few enough tokens, and their features fit in shared memory
+bool takes_few_tokens(int64_t N, int64_t D) { return N <= kFewTokens && (D + 511) / 512 * 512 * kFewTokens * 4 <= 160 * 1024; }
+
 // ------------------------------------------------------------------ joining the tiles' maxima and sums
 
-constexpr int kJoinRows = 32;
-constexpr int kJoinSlices = 8;
+constexpr int kJoinThreads = 256;
 
-// partials [parts][rows] -> maximum, sum and loss per row; with a reduction, the blocks' sums are added up by
-// the block that finishes last, always in the same order.
-__global__ void __launch_bounds__(kJoinRows * kJoinSlices)
+// partials [parts][rows] -> maximum, sum and loss per row, ROWS rows per block; with a reduction, the blocks' sums are
+// added up by the block that finishes last, always in the same order.
+template <int ROWS>
+__global__ void __launch_bounds__(kJoinThreads)
 loss_join_kernel(const float2* __restrict__ partials, const float* __restrict__ target_score,
                  const int64_t* __restrict__ targets, int64_t ignore_index, int64_t vocab, int64_t rows, int parts,
                  int reduction, float* __restrict__ row_max, float* __restrict__ row_sum, float* __restrict__ loss,
                  float* __restrict__ inv_count, double* __restrict__ block_loss, int* __restrict__ block_count,
                  uint32_t* ticket, uint32_t* error_word) {
-  __shared__ float2 s_part[kJoinSlices][kJoinRows];
-  __shared__ double s_loss[kJoinRows * kJoinSlices];
-  __shared__ int s_count[kJoinRows * kJoinSlices];
+  constexpr int kSlices = kJoinThreads / ROWS;
+  __shared__ float2 s_part[kSlices][ROWS];
+  __shared__ double s_loss[kJoinThreads];
+  __shared__ int s_count[kJoinThreads];
   __shared__ bool s_last;
-  const int r = threadIdx.x % kJoinRows, slice = threadIdx.x / kJoinRows;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kJoinRows + r;
-  float mx = -INFINITY, sum = 0.0f;
+  const int r = threadIdx.x % ROWS, slice = threadIdx.x / ROWS;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + r;
+  float2 all = make_float2(-INFINITY, 0.0f);
   if (row < rows) {
-    for (int i = slice; i < parts; i += kJoinSlices) {
-      const float2 q = partials[static_cast<int64_t>(i) * rows + row];
-      const float next = fmaxf(mx, q.x);
-      const float base = next == -INFINITY ? 0.0f : next;
-      sum = sum * exp2_fast(mx - base) + q.y * exp2_fast(q.x - base);
-      mx = next;
+    const float2* src = partials + row;
+    int i = slice;
+    for (; i + 3 * kSlices < parts; i += 4 * kSlices) {
+      float2 q[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) q[e] = src[static_cast<int64_t>(i + e * kSlices) * rows];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) all = join(all, q[e]);
     }
+    for (; i < parts; i += kSlices) all = join(all, src[static_cast<int64_t>(i) * rows]);
   }
-  s_part[slice][r] = make_float2(mx, sum);
+  s_part[slice][r] = all;
   __syncthreads();
+#pragma unroll
+  for (int o = kSlices / 2; o > 0; o >>= 1) {
+    if (slice < o) s_part[slice][r] = join(s_part[slice][r], s_part[slice + o][r]);
+    __syncthreads();
+  }
   float value = 0.0f;
   int counted = 0;
   if (slice == 0 && row < rows) {
-    for (int i = 1; i < kJoinSlices; ++i) {
-      const float2 q = s_part[i][r];
-      const float next = fmaxf(mx, q.x);
-      const float base = next == -INFINITY ? 0.0f : next;
-      sum = sum * exp2_fast(mx - base) + q.y * exp2_fast(q.x - base);
-      mx = next;
-    }
+    const float mx = s_part[0][r].x;
+    float sum = s_part[0][r].y;
     if (mx == -INFINITY) sum = __int_as_float(0x7fc00000);    // every word masked: no distribution
     row_max[row] = mx;
     row_sum[row] = sum;
@@ -157,34 +347,34 @@ loss_join_kernel(const float2* __restrict__ partials, const float* __restrict__ 
     if (reduction == GRMX_REDUCE_NONE) loss[row] = value;
   }
   if (reduction == GRMX_REDUCE_NONE) return;
-  if (slice == 0) {
-    double v = value;
-    int n = counted;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      v += __shfl_xor_sync(0xffffffffu, v, o);
-      n += __shfl_xor_sync(0xffffffffu, n, o);
+  s_loss[threadIdx.x] = value;
+  s_count[threadIdx.x] = counted;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double v = 0.0;
+    int n = 0;
+    for (int i = 0; i < ROWS; ++i) {
+      v += s_loss[i];
+      n += s_count[i];
     }
-    if (r == 0) {
-      block_loss[blockIdx.x] = v;
-      block_count[blockIdx.x] = n;
-      __threadfence();
-      s_last = atomicAdd(ticket, 1u) == gridDim.x - 1;
-    }
+    block_loss[blockIdx.x] = v;
+    block_count[blockIdx.x] = n;
+    __threadfence();
+    s_last = atomicAdd(ticket, 1u) == gridDim.x - 1;
   }
   __syncthreads();
   if (!s_last) return;
   __threadfence();
   double v = 0.0;
   int n = 0;
-  for (unsigned i = threadIdx.x; i < gridDim.x; i += kJoinRows * kJoinSlices) {
+  for (unsigned i = threadIdx.x; i < gridDim.x; i += kJoinThreads) {
     v += __ldcg(block_loss + i);
     n += __ldcg(block_count + i);
   }
   s_loss[threadIdx.x] = v;
   s_count[threadIdx.x] = n;
   __syncthreads();
-  for (int o = kJoinRows * kJoinSlices / 2; o > 0; o >>= 1) {
+  for (int o = kJoinThreads / 2; o > 0; o >>= 1) {
     if (threadIdx.x < o) {
       s_loss[threadIdx.x] += s_loss[threadIdx.x + o];
       s_count[threadIdx.x] += s_count[threadIdx.x + o];
@@ -198,6 +388,9 @@ loss_join_kernel(const float2* __restrict__ partials, const float* __restrict__ 
     *inv_count = reduction == GRMX_REDUCE_MEAN ? (count > 0.0 ? static_cast<float>(1.0 / count) : 0.0f) : 1.0f;
   }
 }
+
+// rows per block: whole lines of the partials where there are rows enough for all SMs, more slices where not
+int join_rows(int64_t N) { return N >= 16384 ? 32 : N >= 512 ? 8 : 1; }
 
 // ------------------------------------------------------------------ sums of partial results
 
@@ -385,6 +578,7 @@ BackwardPlan plan_backward(int64_t N, int64_t D, int64_t V, int dtype, int pairs
 }
 
 struct ForwardPlan {
+  bool few;
   int parts;
   int64_t join_blocks;
   int64_t off_x, off_w, off_part, off_target, off_loss, off_count, off_ticket, bytes;
@@ -392,16 +586,17 @@ struct ForwardPlan {
 
 ForwardPlan plan_forward(int64_t N, int64_t D, int64_t V, int dtype) {
   ForwardPlan f;
-  f.parts = static_cast<int>(ceil_div(V, kTileN)) * parts_of(kEpiLse, dtype == GRMX_F32);
-  f.join_blocks = ceil_div(N, kJoinRows);
+  f.few = takes_few_tokens(N, D);
+  f.parts = f.few ? few_tokens_blocks(V) : static_cast<int>(ceil_div(V, kTileN)) * parts_of(kEpiLse, dtype == GRMX_F32);
+  f.join_blocks = ceil_div(N, join_rows(N));
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     const int64_t here = at;
     at += round_up(bytes, 1024);
     return here;
   };
-  f.off_x = take(operand_bytes(N, D, dtype));
-  f.off_w = take(operand_bytes(V, D, dtype));
+  f.off_x = take(f.few ? 0 : operand_bytes(N, D, dtype));
+  f.off_w = take(f.few ? 0 : operand_bytes(V, D, dtype));
   f.off_part = take(f.parts * N * 8);
   f.off_target = take(N * 4);
   f.off_loss = take(f.join_blocks * 8);
@@ -461,36 +656,46 @@ extern "C" int grmx_linear_xent_fwd(const void* hidden, const void* weight, cons
   GRMX_TRY(check_device(who));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  Operand x, w;
-  uint8_t* at = ws + f.off_x;
-  GRMX_TRY(make_operand(&x, hidden, N, D, dtype, &at, s));
-  at = ws + f.off_w;
-  GRMX_TRY(make_operand(&w, weight, V, D, dtype, &at, s));
-  Maps maps;
-  if (!operand_map(&maps.a, x, N, D, false) || !operand_map(&maps.b, w, V, D, false)) {
-    return fail(GRMX_ERR_LAUNCH, "%s: cuTensorMapEncodeTiled failed", who);
+  float2* partials = reinterpret_cast<float2*>(ws + f.off_part);
+  float* target_score = reinterpret_cast<float*>(ws + f.off_target);
+  uint32_t* ticket = reinterpret_cast<uint32_t*>(ws + f.off_ticket);
+  if (f.few) {
+    const int n = static_cast<int>(N), d = static_cast<int>(D);
+    GRMX_TRY(dtype == GRMX_F32 ? launch_few_tokens<float>(hidden, weight, bias, bias_dtype, targets, ignore_index, n, d, V, partials, target_score, ticket, s)
+                               : launch_few_tokens<__nv_bfloat16>(hidden, weight, bias, bias_dtype, targets, ignore_index, n, d, V, partials, target_score, ticket, s));
+  } else {
+    Operand x, w;
+    uint8_t* at = ws + f.off_x;
+    GRMX_TRY(make_operand(&x, hidden, N, D, dtype, &at, s));
+    at = ws + f.off_w;
+    GRMX_TRY(make_operand(&w, weight, V, D, dtype, &at, s));
+    Maps maps;
+    if (!operand_map(&maps.a, x, N, D, false) || !operand_map(&maps.b, w, V, D, false)) {
+      return fail(GRMX_ERR_LAUNCH, "%s: cuTensorMapEncodeTiled failed", who);
+    }
+    maps.c = maps.a;
+    Params p;
+    memset(&p, 0, sizeof(p));
+    p.m_tiles = static_cast<int>(ceil_div(N, kTileM));
+    p.n_tiles = static_cast<int>(ceil_div(V, kTileN));
+    p.splits = 1;
+    p.k_blocks = p.blocks_per_split = static_cast<int>(ceil_div(D, kBlockK));
+    p.rows = N;
+    p.cols = V;
+    p.vocab = V;
+    p.bias = bias;
+    p.bias_dtype = bias_dtype;
+    p.targets = targets;
+    p.ignore_index = ignore_index;
+    p.partials = partials;
+    p.target_score = target_score;
+    p.ticket = ticket;
+    GRMX_TRY(launch_scores<kEpiLse>(maps, p, dtype, "loss scores", s));
   }
-  maps.c = maps.a;
-  Params p;
-  memset(&p, 0, sizeof(p));
-  p.m_tiles = static_cast<int>(ceil_div(N, kTileM));
-  p.n_tiles = static_cast<int>(ceil_div(V, kTileN));
-  p.splits = 1;
-  p.k_blocks = p.blocks_per_split = static_cast<int>(ceil_div(D, kBlockK));
-  p.rows = N;
-  p.cols = V;
-  p.vocab = V;
-  p.bias = bias;
-  p.bias_dtype = bias_dtype;
-  p.targets = targets;
-  p.ignore_index = ignore_index;
-  p.partials = reinterpret_cast<float2*>(ws + f.off_part);
-  p.target_score = reinterpret_cast<float*>(ws + f.off_target);
-  p.ticket = reinterpret_cast<uint32_t*>(ws + f.off_ticket);
-  GRMX_TRY(launch_scores<kEpiLse>(maps, p, dtype, "loss scores", s));
-  loss_join_kernel<<<static_cast<unsigned>(f.join_blocks), kJoinRows * kJoinSlices, 0, s>>>(
-      p.partials, p.target_score, targets, ignore_index, V, N, f.parts, reduction, row_stats, row_stats + N, loss, inv_count,
-      reinterpret_cast<double*>(ws + f.off_loss), reinterpret_cast<int*>(ws + f.off_count), p.ticket, device_error_word_ptr());
+  auto join_kernel = join_rows(N) == 32 ? loss_join_kernel<32> : join_rows(N) == 8 ? loss_join_kernel<8> : loss_join_kernel<1>;
+  join_kernel<<<static_cast<unsigned>(f.join_blocks), kJoinThreads, 0, s>>>(
+      partials, target_score, targets, ignore_index, V, N, f.parts, reduction, row_stats, row_stats + N, loss, inv_count,
+      reinterpret_cast<double*>(ws + f.off_loss), reinterpret_cast<int*>(ws + f.off_count), ticket, device_error_word_ptr());
   return check_launch("loss join");
 }
 
