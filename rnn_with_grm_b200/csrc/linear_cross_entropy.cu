@@ -747,7 +747,12 @@ extern "C" int grmx_linear_xent_bwd(const float* grad_loss, const void* hidden, 
     const int64_t v0 = piece * b.piece;
     const int64_t words = V - v0 < b.piece ? V - v0 : b.piece;       // of the vocabulary in this piece
     const int64_t width = round_up(words, kTileN);
-    const Operand d{ws + b.off_d, b.piece, N * b.piece, planes};
+    const int panels = static_cast<int>(width / 64);
+    const void* d = ws + b.off_d;
+    // boxes of 64 columns x 128 rows (d as it is) or x 64 rows (d transposed)
+    auto d_map = [&](CUtensorMap* map, int rows) {
+      return make_matrix_map(map, d, false, static_cast<int64_t>(planes) * panels, N, 64, 64, N * 64, 64, rows);
+    };
     const Operand w_piece{static_cast<const uint8_t*>(w.ptr) + v0 * w.ld * 2, w.ld, w.plane_stride, w.planes};
     {
       Maps maps;
@@ -758,8 +763,7 @@ extern "C" int grmx_linear_xent_bwd(const float* grad_loss, const void* hidden, 
       Params p;
       memset(&p, 0, sizeof(p));
       p.d_out = reinterpret_cast<__nv_bfloat16*>(ws + b.off_d);
-      p.d_ld = d.ld;
-      p.d_plane_stride = d.plane_stride;
+      p.panels = panels;
       p.m_tiles = static_cast<int>(ceil_div(N, kTileM));
       p.n_tiles = static_cast<int>(width / kTileN);
       p.splits = 1;
@@ -794,7 +798,7 @@ extern "C" int grmx_linear_xent_bwd(const float* grad_loss, const void* hidden, 
       Maps maps;
       const bool to_f32 = f32 || !direct_x;
       const int64_t ld = direct_x ? D : b.pitch;
-      if (!operand_map(&maps.a, d, N, width, false) || !operand_map(&maps.b, w_piece, words, D, true) ||
+      if (!d_map(&maps.a, 128) || !operand_map(&maps.b, w_piece, words, D, true) ||
           !make_matrix_map(&maps.c, direct_x ? grad_hidden : part_x, to_f32, b.splits_x, N, D, ld, N * ld, to_f32 ? 32 : 64, 128)) {
         return fail(GRMX_ERR_LAUNCH, "%s: cuTensorMapEncodeTiled failed", who);
       }
@@ -808,6 +812,7 @@ extern "C" int grmx_linear_xent_bwd(const float* grad_loss, const void* hidden, 
       p.splits = static_cast<int>(ceil_div(p.k_blocks, p.blocks_per_split));
       p.rows = N;
       p.cols = D;
+      p.panels = panels;
       p.store_f32 = to_f32;
       p.store_add = piece > 0;
       p.scale = scale;
@@ -821,7 +826,7 @@ extern "C" int grmx_linear_xent_bwd(const float* grad_loss, const void* hidden, 
       const bool to_f32 = f32 || !direct_w;
       const int64_t ld = direct_w ? D : b.pitch;
       void* out = static_cast<uint8_t*>(grad_weight) + v0 * D * elem;
-      if (!operand_map(&maps.a, d, N, width, true) || !operand_map(&maps.b, x, N, D, true) ||
+      if (!d_map(&maps.a, 64) || !operand_map(&maps.b, x, N, D, true) ||
           !make_matrix_map(&maps.c, direct_w ? out : part_w, to_f32, b.splits_w, words, D, ld, b.piece * ld, to_f32 ? 32 : 64, 128)) {
         return fail(GRMX_ERR_LAUNCH, "%s: cuTensorMapEncodeTiled failed", who);
       }
@@ -834,6 +839,7 @@ extern "C" int grmx_linear_xent_bwd(const float* grad_loss, const void* hidden, 
       p.splits = b.splits_w;
       p.rows = words;
       p.cols = D;
+      p.panels = panels;
       p.store_f32 = to_f32;
       p.scale = scale;
       p.scale2 = scale2;

@@ -74,7 +74,7 @@ def within(got, want, tol, what):
 
 
 SHAPES = [(1, 1, 1), (1, 512, 1000), (2, 64, 256), (7, 33, 257), (127, 65, 255), (129, 8, 300), (256, 128, 512), (300, 72, 513),
-          (513, 520, 777), (40, 1030, 130), (3, 100, 33), (8, 520, 3000), (9, 520, 3000), (4, 6000, 70)]
+          (513, 520, 777), (40, 1030, 130), (3, 100, 33), (8, 520, 3000), (9, 520, 3000), (4, 6000, 70), (260, 257, 300), (260, 384, 300), (260, 385, 300)]
 
 
 @pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "x".join(map(str, s)))
