@@ -101,6 +101,96 @@ __device__ __forceinline__ void sigmoid_pair(float g, float& yes, float& no) {
   no = g >= 0.0f ? small : r;
 }
 
+// ---- arithmetic on a piece: two values per instruction for the eight of a bf16 piece; fp32 pieces keep to single ones,
+// where pairs cost registers (backward 16384 x 1024 with scale and sum: 92 us single, 103 paired) ----
+__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+// x = x * m + a, x = x * m, x = x + a over VEC values
+template <int VEC>
+__device__ __forceinline__ void fma_all(float (&x)[VEC], const float (&m)[VEC], const float (&a)[VEC]) {
+  if constexpr (VEC < 8) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) x[j] = fmaf(x[j], m[j], a[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC; j += 2) {
+      uint64_t r;
+      asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(pack2(x[j], x[j + 1])), "l"(pack2(m[j], m[j + 1])), "l"(pack2(a[j], a[j + 1])));
+      unpack2(r, x[j], x[j + 1]);
+    }
+  }
+}
+template <int VEC>
+__device__ __forceinline__ void mul_all(float (&x)[VEC], const float (&m)[VEC]) {
+  if constexpr (VEC < 8) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) x[j] *= m[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC; j += 2) {
+      uint64_t r;
+      asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pack2(x[j], x[j + 1])), "l"(pack2(m[j], m[j + 1])));
+      unpack2(r, x[j], x[j + 1]);
+    }
+  }
+}
+template <int VEC>
+__device__ __forceinline__ void add_all(float (&x)[VEC], const float (&a)[VEC]) {
+  if constexpr (VEC < 8) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) x[j] += a[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC; j += 2) {
+      uint64_t r;
+      asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pack2(x[j], x[j + 1])), "l"(pack2(a[j], a[j + 1])));
+      unpack2(r, x[j], x[j + 1]);
+    }
+  }
+}
+// sums += x * y
+template <int VEC>
+__device__ __forceinline__ void add_products(float (&sums)[VEC], const float (&x)[VEC], const float (&y)[VEC]) {
+  if constexpr (VEC < 8) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) sums[j] = fmaf(x[j], y[j], sums[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC; j += 2) {
+      uint64_t r;
+      asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(pack2(x[j], x[j + 1])), "l"(pack2(y[j], y[j + 1])), "l"(pack2(sums[j], sums[j + 1])));
+      unpack2(r, sums[j], sums[j + 1]);
+    }
+  }
+}
+// sums += x * x
+template <int VEC>
+__device__ __forceinline__ void add_squares(float (&sums)[VEC], const float (&x)[VEC]) {
+  if constexpr (VEC < 8) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) sums[j] = fmaf(x[j], x[j], sums[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC; j += 2) {
+      const uint64_t v = pack2(x[j], x[j + 1]);
+      uint64_t r;
+      asm("fma.rn.f32x2 %0, %1, %1, %2;" : "=l"(r) : "l"(v), "l"(pack2(sums[j], sums[j + 1])));
+      unpack2(r, sums[j], sums[j + 1]);
+    }
+  }
+}
+template <int VEC>
+__device__ __forceinline__ void fill_all(float (&x)[VEC], float v) {
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) x[j] = v;
+}
+
 // Sums over the G threads of a row; all of them get the result.  `turn` alternates between two places for the warps'
 // parts: whoever writes to one of them has passed the barrier that followed the last read of it.
 template <int G>
@@ -282,8 +372,8 @@ fuse_norm_fwd_kernel(const __grid_constant__ RowArgs a) {
         if (GATE) load_piece<T, VEC, ACCESS>(rg[i], a.gate, base, col.at(i), col.live(i), total);
       }
     }
-    float s[kPieces][VEC];
-    float sum = 0.0f;
+    float s[kPieces][VEC], part[VEC];
+    fill_all(part, 0.0f);
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
       if (i < col.count) {
@@ -293,37 +383,52 @@ fuse_norm_fwd_kernel(const __grid_constant__ RowArgs a) {
         ru[i].unpack(u);
         if (a.scale != nullptr) {
           load_param<VEC, ACCESS>(a, a.scale, p_scale, col.at(i), 1.0f, k);
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) u[j] *= k[j];
+          mul_all(u, k);
         }
-        if (GATE) rg[i].unpack(k);
+        if (GATE) {
+          float yes[VEC];
+          rg[i].unpack(k);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          if (GATE) {
-            float yes, no;
-            sigmoid_pair(k[j], yes, no);
-            s[i][j] = fmaf(yes, o[j], no * u[j]);
-          } else {
-            s[i][j] = o[j] + u[j];
+          for (int j = 0; j < VEC; ++j) {
+            float no;
+            sigmoid_pair(k[j], yes[j], no);
+            k[j] = no;
           }
-          if (live && col.holds(col.at(i) + j)) sum += s[i][j];
+          mul_all(u, k);
+          fma_all(o, yes, u);
+        } else {
+          add_all(o, u);
         }
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) s[i][j] = live && col.holds(col.at(i) + j) ? o[j] : 0.0f;
+        add_all(part, s[i]);
         if (a.sum_out != nullptr) store_piece<T>(a.sum_out, base, col, i, s[i]);
       }
     }
+    float sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) sum += part[j];
     const float mean = row_sum<G>(sum, s_scratch[group], turn) * inv;
-    sum = 0.0f;
+    float minus[VEC];
+    fill_all(minus, -mean);
+    fill_all(part, 0.0f);
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
-      if (i < col.count && col.live(i)) {
+      if (i < col.count) {
+        add_all(s[i], minus);
+        if (ACCESS == kShifted || !col.live(i)) {            // what is not of the row does not count
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const float d = s[i][j] - mean;
-          if (col.holds(col.at(i) + j)) sum = fmaf(d, d, sum);
+          for (int j = 0; j < VEC; ++j) s[i][j] = col.live(i) && col.holds(col.at(i) + j) ? s[i][j] : 0.0f;
         }
+        add_squares(part, s[i]);
       }
     }
+    sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) sum += part[j];
     const float rstd = rsqrtf(row_sum<G>(sum, s_scratch[group], turn) * inv + a.eps);
+    float scale_by[VEC];
+    fill_all(scale_by, rstd);
     if (lane == 0 && a.stats != nullptr) a.stats[row] = make_float2(mean, rstd);
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
@@ -331,8 +436,8 @@ fuse_norm_fwd_kernel(const __grid_constant__ RowArgs a) {
         float w[VEC], b[VEC];
         load_param<VEC, ACCESS>(a, a.weight, p_weight, col.at(i), 1.0f, w);
         load_param<VEC, ACCESS>(a, a.bias, p_bias, col.at(i), 0.0f, b);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) s[i][j] = fmaf((s[i][j] - mean) * rstd, w[j], b[j]);
+        mul_all(s[i], scale_by);
+        fma_all(s[i], w, b);
         store_piece<T>(a.out, base, col, i, s[i]);
       }
     }
@@ -379,94 +484,124 @@ fuse_norm_bwd_kernel(const __grid_constant__ RowArgs a) {
         if (GATE) load_piece<T, VEC, ACCESS>(rg[i], a.gate, base, col.at(i), col.live(i), total);
       }
     }
-    float xh[kPieces][VEC], da[kPieces][VEC];
+    float xh[kPieces][VEC], da[kPieces][VEC], part[VEC], part_xh[VEC], minus[VEC], by[VEC];
     float2 sum = make_float2(0.0f, 0.0f);
+    fill_all(part, 0.0f);
+    fill_all(part_xh, 0.0f);
+    fill_all(minus, -st.x);
+    fill_all(by, st.y);
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
       if (i < col.count) {
-        const bool live = col.live(i);
-        float o[VEC], u[VEC], k[VEC], w[VEC];
-        ro[i].unpack(o);
+        float u[VEC], k[VEC];
+        ro[i].unpack(xh[i]);
         ru[i].unpack(u);
         if (SCALE) {
           load_param<VEC, ACCESS>(a, a.scale, p_scale, col.at(i), 1.0f, k);
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) u[j] *= k[j];
+          mul_all(u, k);
         }
-        if (GATE) rg[i].unpack(k);
+        if (GATE) {
+          float yes[VEC];
+          rg[i].unpack(k);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          float s;
-          if (GATE) {
-            float yes, no;
-            sigmoid_pair(k[j], yes, no);
-            s = fmaf(yes, o[j], no * u[j]);
-          } else {
-            s = o[j] + u[j];
+          for (int j = 0; j < VEC; ++j) {
+            float no;
+            sigmoid_pair(k[j], yes[j], no);
+            k[j] = no;
           }
-          xh[i][j] = (s - st.x) * st.y;
+          mul_all(u, k);
+          fma_all(xh[i], yes, u);
+        } else {
+          add_all(xh[i], u);
         }
-        load_param<VEC, ACCESS>(a, a.weight, p_weight, col.at(i), 1.0f, w);
+        add_all(xh[i], minus);
+        mul_all(xh[i], by);
         if (have_dy) {
-          rd[i].unpack(o);
+          rd[i].unpack(da[i]);
+        } else {
+          fill_all(da[i], 0.0f);
+        }
+        if (ACCESS == kShifted || !col.live(i)) {              // what is not of the row does not count
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) {
+            const bool counts = col.live(i) && col.holds(col.at(i) + j);
+            xh[i][j] = counts ? xh[i][j] : 0.0f;
+            da[i][j] = counts ? da[i][j] : 0.0f;
+          }
+        }
+        add_products(cw[i], da[i], xh[i]);
+        add_all(cb[i], da[i]);
+        load_param<VEC, ACCESS>(a, a.weight, p_weight, col.at(i), 1.0f, k);
+        mul_all(da[i], k);
+        if constexpr (VEC == 8) {
+          add_all(part, da[i]);
+          add_products(part_xh, da[i], xh[i]);
         } else {
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) o[j] = 0.0f;
-        }
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          da[i][j] = o[j] * w[j];
-          if (live && col.holds(col.at(i) + j)) {
-            cw[i][j] = fmaf(o[j], xh[i][j], cw[i][j]);
-            cb[i][j] += o[j];
+          for (int j = 0; j < VEC; ++j) {
             sum.x += da[i][j];
             sum.y = fmaf(da[i][j], xh[i][j], sum.y);
           }
         }
       }
     }
+    if constexpr (VEC == 8) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        sum.x += part[j];
+        sum.y += part_xh[j];
+      }
+    }
     sum = row_sum2<G>(sum, s_scratch[group], turn);
-    const float m1 = sum.x * inv, m2 = sum.y * inv;
+    float minus_xh[VEC];
+    fill_all(minus, -sum.x * inv);
+    fill_all(minus_xh, -sum.y * inv);
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
       if (i < col.count) {
-        const bool live = col.live(i);
-        float ds[VEC], dv[VEC], u[VEC], k[VEC];
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) ds[j] = st.y * (da[i][j] - m1 - xh[i][j] * m2);
+        float dv[VEC], u[VEC], k[VEC];
+        float (&ds)[VEC] = da[i];
+        add_products(ds, xh[i], minus_xh);
+        add_all(ds, minus);
+        mul_all(ds, by);
         if (a.grad_sum != nullptr) {
           Raw<T, VEC> raw;
-          load_piece<T, VEC, ACCESS>(raw, a.grad_sum, base, col.at(i), live, total);
+          load_piece<T, VEC, ACCESS>(raw, a.grad_sum, base, col.at(i), col.live(i), total);
           raw.unpack(dv);
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) ds[j] += dv[j];
+          add_all(ds, dv);
         }
-        if (SCALE) load_param<VEC, ACCESS>(a, a.scale, p_scale, col.at(i), 1.0f, k);
         ru[i].unpack(u);
+        if (SCALE) load_param<VEC, ACCESS>(a, a.scale, p_scale, col.at(i), 1.0f, k);
         if (GATE) {
-          float o[VEC], g[VEC], dg[VEC];
-          ro[i].unpack(o);
+          float dg[VEC], g[VEC], yes[VEC], other[VEC];
+          // online - scale update
+          ro[i].unpack(dg);
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) other[j] = SCALE ? -k[j] : -1.0f;
+          add_products(dg, u, other);
           rg[i].unpack(g);
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            float yes, no;
-            sigmoid_pair(g[j], yes, no);
-            dg[j] = ds[j] * (o[j] - (SCALE ? u[j] * k[j] : u[j])) * (yes * no);
-            dv[j] = ds[j] * no;
-            ds[j] *= yes;
-          }
+          for (int j = 0; j < VEC; ++j) sigmoid_pair(g[j], yes[j], dv[j]);
+          mul_all(dg, ds);
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) other[j] = yes[j];
+          mul_all(other, dv);
+          mul_all(dg, other);
+          mul_all(dv, ds);
+          mul_all(ds, yes);
           if (a.grad_gate != nullptr) store_piece<T>(a.grad_gate, base, col, i, dg);
         } else {
 #pragma unroll
           for (int j = 0; j < VEC; ++j) dv[j] = ds[j];
         }
         if (a.grad_online != nullptr) store_piece<T>(a.grad_online, base, col, i, ds);
-        if (SCALE) {
+        if constexpr (SCALE) {
+          if (ACCESS == kShifted || !col.live(i)) {
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            if (live && col.holds(col.at(i) + j)) cs[SCALE ? i : 0][j] = fmaf(dv[j], u[j], cs[SCALE ? i : 0][j]);
-            dv[j] *= k[j];
+            for (int j = 0; j < VEC; ++j) u[j] = col.live(i) && col.holds(col.at(i) + j) ? u[j] : 0.0f;
           }
+          add_products(cs[i], dv, u);
+          mul_all(dv, k);
         }
         if (a.grad_update != nullptr) store_piece<T>(a.grad_update, base, col, i, dv);
       }
@@ -544,19 +679,19 @@ int sm_count() {
 
 // `width`: a row's values, and for shifted rows what a piece may stick out by
 int threads_per_row(int64_t width, int values) {
-  for (int G : {32, 64, 128, 256}) {
+  for (int G : {32, 64, 128, 256, 512}) {
     if (width <= G * values) return G;
   }
   return 1024;
 }
 enum { kSlack = 7 };           // values of a 16-byte piece that may lie before a shifted row
 
-// CTAs of a backward pass: three per SM (one of 1024 threads), or as many as there are rows; a multiple of eight row
+// CTAs of a backward pass: three per SM (two of 512 threads, one of 1024), or as many as there are rows; a multiple of eight row
 // groups, so that a thread's rows all start at the same place of a 16-byte piece
 int64_t backward_ctas(int64_t rows, int G) {
   const int64_t per = threads_of(G) / G, unit = per >= 8 ? 1 : 8 / per;
   const int64_t need = (rows + per - 1) / per;
-  const int64_t most = (G > 256 ? 1 : 3) * static_cast<int64_t>(sm_count()) / unit * unit;
+  const int64_t most = (G > 512 ? 1 : G > 256 ? 2 : 3) * static_cast<int64_t>(sm_count()) / unit * unit;
   return need < most ? (need + unit - 1) / unit * unit : most;
 }
 // of either way to see the rows: the workspace is sized before the pointers are known
@@ -580,8 +715,8 @@ int launch_group(const RowArgs& a, bool backward, cudaStream_t s) {
   if (!backward) {
     constexpr int64_t kUnit = kGroups >= 8 ? 1 : 8 / kGroups;
     int64_t grid = ((a.rows + kGroups - 1) / kGroups + kUnit - 1) / kUnit * kUnit;
-    // shifted rows stage the parameters once per CTA: a CTA lives for several rows
-    const int64_t most = (ACCESS == kShifted ? 4 * static_cast<int64_t>(sm_count()) : 0x7ffffff0LL) / kUnit * kUnit;
+    // a CTA lives for several rows (its set-up costs a fifth of a row of 512)
+    const int64_t most = (G > 256 ? 2 : 6) * static_cast<int64_t>(sm_count()) / kUnit * kUnit;
     if (grid > most) grid = most;
     const int smem = ACCESS == kShifted ? 3 * staged_words(a.H) * 4 : 0;
     return a.gate != nullptr ? launch_rows(fuse_norm_fwd_kernel<T, VEC, G, ACCESS, true>, a, grid, threads_of(G), smem, "fuse_norm", s)
@@ -603,6 +738,7 @@ int launch_width(const RowArgs& a, bool backward, cudaStream_t s) {
     case 64: return launch_group<T, VEC, 64, ACCESS>(a, backward, s);
     case 128: return launch_group<T, VEC, 128, ACCESS>(a, backward, s);
     case 256: return launch_group<T, VEC, 256, ACCESS>(a, backward, s);
+    case 512: return launch_group<T, VEC, 512, ACCESS>(a, backward, s);
     default: return launch_group<T, VEC, 1024, ACCESS>(a, backward, s);
   }
 }

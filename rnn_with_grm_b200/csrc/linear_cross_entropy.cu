@@ -34,10 +34,16 @@ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // [rows, cols] fp32 or bf16 -> planes of bf16 whose sum is the value (one plane for bf16: a copy with a pitch
 // that a tensor map can take).  x = h + m + l with h = bf16(x), m = bf16(x - h), l = bf16(x - h - m): 24 bits.
-// Values that are not finite stay whole in the first plane.
+// Values that are not finite stay whole in the first plane.  With targets the rows are tokens: one that does not
+// count becomes zeros (whatever it holds), the others are multiplied by grad[row] if there is such a factor.
+struct TokenRows {
+  const int64_t* targets;      // NULL: plain rows
+  int64_t ignore_index, vocab;
+  const float* grad;           // [rows] or NULL
+};
 template <typename T, int PLANES>
 __global__ void __launch_bounds__(256) planes_kernel(const T* __restrict__ src, __nv_bfloat16* __restrict__ dst, int64_t rows,
-                                                     int cols, int ld, int64_t plane_stride) {
+                                                     int cols, int ld, int64_t plane_stride, TokenRows tokens) {
   const int64_t pairs = ld / 2;
   const int64_t total = rows * pairs;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * 256) {
@@ -46,6 +52,13 @@ __global__ void __launch_bounds__(256) planes_kernel(const T* __restrict__ src, 
     float v[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) v[e] = c + e < cols ? to_float<T>(src[r * cols + c + e]) : 0.0f;
+    if (tokens.targets != nullptr) {
+      const int64_t t = __ldg(tokens.targets + r);
+      const bool counts = t != tokens.ignore_index && t >= 0 && t < tokens.vocab;
+      const float factor = tokens.grad != nullptr ? __ldg(tokens.grad + r) : 1.0f;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) v[e] = counts ? v[e] * factor : 0.0f;
+    }
 #pragma unroll
     for (int pl = 0; pl < PLANES; ++pl) {
       __nv_bfloat162 b;
@@ -76,29 +89,32 @@ int64_t operand_bytes(int64_t rows, int64_t cols, int dtype) {
   return (dtype == GRMX_F32 ? 3 : 1) * round_up(rows * round_up(cols, 8) * 2, 256);
 }
 
-int make_operand(Operand* out, const void* src, int64_t rows, int64_t cols, int dtype, uint8_t** ws, cudaStream_t s) {
-  const int64_t bytes = operand_bytes(rows, cols, dtype);
-  uint8_t* dst = *ws;
-  *ws += bytes;
-  if (readable_in_place(src, cols, dtype)) {
-    *out = Operand{src, cols, rows * cols, 1};
-    return GRMX_OK;
-  }
+// Always a copy, in planes, at dst (operand_bytes of it).
+int copy_operand(Operand* out, const void* src, int64_t rows, int64_t cols, int dtype, uint8_t* dst, const TokenRows& tokens,
+                 cudaStream_t s) {
   const int64_t ld = round_up(cols, 8);
   const int planes = dtype == GRMX_F32 ? 3 : 1;
-  const int64_t stride = bytes / planes / 2;
+  const int64_t stride = operand_bytes(rows, cols, dtype) / planes / 2;
   const int64_t blocks = ceil_div(rows * (ld / 2), 256);
   const unsigned grid = static_cast<unsigned>(blocks < 148 * 16 ? blocks : 148 * 16);
   __nv_bfloat16* d = reinterpret_cast<__nv_bfloat16*>(dst);
   if (dtype == GRMX_F32) {
     planes_kernel<float, 3><<<grid, 256, 0, s>>>(static_cast<const float*>(src), d, rows, static_cast<int>(cols),
-                                                  static_cast<int>(ld), stride);
+                                                  static_cast<int>(ld), stride, tokens);
   } else {
     planes_kernel<__nv_bfloat16, 1><<<grid, 256, 0, s>>>(static_cast<const __nv_bfloat16*>(src), d, rows,
-                                                          static_cast<int>(cols), static_cast<int>(ld), stride);
+                                                          static_cast<int>(cols), static_cast<int>(ld), stride, tokens);
   }
   *out = Operand{dst, ld, stride, planes};
   return check_launch("loss operand planes");
+}
+// The matrix as it is where a tensor map can read it, otherwise a copy.
+int make_operand(Operand* out, const void* src, int64_t rows, int64_t cols, int dtype, uint8_t* dst, cudaStream_t s) {
+  if (readable_in_place(src, cols, dtype)) {
+    *out = Operand{src, cols, rows * cols, 1};
+    return GRMX_OK;
+  }
+  return copy_operand(out, src, rows, cols, dtype, dst, TokenRows{nullptr, 0, 0, nullptr}, s);
 }
 
 // ------------------------------------------------------------------ a few tokens
@@ -541,7 +557,7 @@ struct BackwardPlan {
   int pieces;
   int splits_x, splits_w;
   int64_t pitch;               // of the fp32 partial results
-  int64_t off_x, off_w, off_d, off_dx, off_dw, off_bias, bytes;
+  int64_t off_x, off_w, off_xc, off_d, off_dx, off_dw, off_bias, bytes;
 };
 
 constexpr int64_t kPieceBytes = int64_t(1) << 30;            // most of the gradient of the scores that is held at a time
@@ -569,6 +585,7 @@ BackwardPlan plan_backward(int64_t N, int64_t D, int64_t V, int dtype, int pairs
   };
   b.off_x = take(operand_bytes(N, D, dtype));
   b.off_w = take(operand_bytes(V, D, dtype));
+  b.off_xc = take(operand_bytes(N, D, dtype));
   b.off_d = take(planes * N * b.piece * 2);
   b.off_dx = take(b.splits_x * N * b.pitch * 4);
   b.off_dw = take(b.splits_w * b.piece * b.pitch * 4);
@@ -665,10 +682,8 @@ extern "C" int grmx_linear_xent_fwd(const void* hidden, const void* weight, cons
                                : launch_few_tokens<__nv_bfloat16>(hidden, weight, bias, bias_dtype, targets, ignore_index, n, d, V, partials, target_score, ticket, s));
   } else {
     Operand x, w;
-    uint8_t* at = ws + f.off_x;
-    GRMX_TRY(make_operand(&x, hidden, N, D, dtype, &at, s));
-    at = ws + f.off_w;
-    GRMX_TRY(make_operand(&w, weight, V, D, dtype, &at, s));
+    GRMX_TRY(make_operand(&x, hidden, N, D, dtype, ws + f.off_x, s));
+    GRMX_TRY(make_operand(&w, weight, V, D, dtype, ws + f.off_w, s));
     Maps maps;
     if (!operand_map(&maps.a, x, N, D, false) || !operand_map(&maps.b, w, V, D, false)) {
       return fail(GRMX_ERR_LAUNCH, "%s: cuTensorMapEncodeTiled failed", who);
@@ -725,19 +740,23 @@ extern "C" int grmx_linear_xent_bwd(const float* grad_loss, const void* hidden, 
   const int planes = f32 ? 3 : 1;
   const int64_t elem = f32 ? 4 : 2;
   Operand x, w;
-  uint8_t* at = ws + b.off_x;
-  GRMX_TRY(make_operand(&x, hidden, N, D, dtype, &at, s));
-  at = ws + b.off_w;
-  GRMX_TRY(make_operand(&w, weight, V, D, dtype, &at, s));
+  GRMX_TRY(make_operand(&x, hidden, N, D, dtype, ws + b.off_x, s));
+  GRMX_TRY(make_operand(&w, weight, V, D, dtype, ws + b.off_w, s));
   const int n_tiles_d = static_cast<int>(ceil_div(D, kTileN));
   float* part_x = reinterpret_cast<float*>(ws + b.off_dx);
   float* part_w = reinterpret_cast<float*>(ws + b.off_dw);
   float* part_b = reinterpret_cast<float*>(ws + b.off_bias);
-  // A factor that all tokens share (the upstream gradient of a sum or a mean, 1 / count) multiplies the finished
-  // sums: d is then p - [target] itself, and the -1 of a target, which carries most of the gradient, is exact in
-  // bf16 where p is small.  A factor per token has to go into d before it is rounded.
-  const float* scale = reduction == GRMX_REDUCE_NONE ? nullptr : grad_loss;
+  // d is held as p - [target] without its factor: the -1 of a target, which carries most of the gradient, is then exact
+  // in bf16 where p is small.  A factor that all tokens share (the upstream gradient of a sum or a mean, 1 / count)
+  // multiplies the finished sums.  A factor per token multiplies the finished rows of dx, goes into the sums of db, and
+  // for dW into a copy of the tokens, in which tokens that do not count are zeros: nothing that they hold reaches dW.
+  const bool per_row = reduction == GRMX_REDUCE_NONE;
+  const float* scale = per_row ? nullptr : grad_loss;
   const float* scale2 = reduction == GRMX_REDUCE_MEAN ? inv_count : nullptr;
+  Operand x_counted;
+  if (grad_weight != nullptr) {
+    GRMX_TRY(copy_operand(&x_counted, hidden, N, D, dtype, ws + b.off_xc, TokenRows{targets, ignore_index, V, per_row ? grad_loss : nullptr}, s));
+  }
   // a result that is complete after one product leaves its epilogue in the caller's type
   auto storable = [&](const void* out) { return D * elem % 16 == 0 && (reinterpret_cast<uintptr_t>(out) & 15u) == 0; };
   const bool direct_x = b.pieces == 1 && b.splits_x == 1 && storable(grad_hidden);
@@ -778,7 +797,7 @@ extern "C" int grmx_linear_xent_bwd(const float* grad_loss, const void* hidden, 
       p.ignore_index = ignore_index;
       p.row_max = row_stats;
       p.row_sum = row_stats + N;
-      p.grad = reduction == GRMX_REDUCE_NONE ? grad_loss : nullptr;
+      p.grad = per_row ? grad_loss : nullptr;
       p.bias_partials = grad_bias != nullptr ? part_b : nullptr;
       GRMX_TRY(launch_scores<kEpiGrad>(maps, p, dtype, "loss score gradient", s));
     }
@@ -815,6 +834,10 @@ extern "C" int grmx_linear_xent_bwd(const float* grad_loss, const void* hidden, 
       p.panels = panels;
       p.store_f32 = to_f32;
       p.store_add = piece > 0;
+      p.grad = per_row ? grad_loss : nullptr;
+      p.targets = targets;
+      p.ignore_index = ignore_index;
+      p.vocab = V;
       p.scale = scale;
       p.scale2 = scale2;
       GRMX_TRY(f32 ? (launch_pair<kEpiStore, false, true, true>(maps, p, "loss hidden gradient", s))
@@ -826,7 +849,7 @@ extern "C" int grmx_linear_xent_bwd(const float* grad_loss, const void* hidden, 
       const bool to_f32 = f32 || !direct_w;
       const int64_t ld = direct_w ? D : b.pitch;
       void* out = static_cast<uint8_t*>(grad_weight) + v0 * D * elem;
-      if (!d_map(&maps.a, 64) || !operand_map(&maps.b, x, N, D, true) ||
+      if (!d_map(&maps.a, 64) || !operand_map(&maps.b, x_counted, N, D, true) ||
           !make_matrix_map(&maps.c, direct_w ? out : part_w, to_f32, b.splits_w, words, D, ld, b.piece * ld, to_f32 ? 32 : 64, 128)) {
         return fail(GRMX_ERR_LAUNCH, "%s: cuTensorMapEncodeTiled failed", who);
       }

@@ -50,8 +50,9 @@ constexpr int kOffMisc = kOffBars + kNumBars * 8;
 constexpr int kSmemTotal = kOffMisc + 32;
 static_assert(kSmemTotal <= kSmemAlloc, "shared memory plan exceeds 227 KiB");
 static_assert(kOffBars % 8 == 0, "barriers are 8-byte aligned");
-// k blocks between two drains of the accumulator in full precision: 32 blocks are 128 accumulations
-constexpr int kSegmentSteps = 32;
+// k blocks between two drains of the accumulator in full precision: 8 blocks are 32 accumulations (the tensor core's
+// additions drop what falls off: with 128 between drains dW of 2048 tokens was 1.6e-6 off, twice what fp32 sums are)
+constexpr int kSegmentSteps = 8;
 
 enum Epilogue { kEpiLse = 0, kEpiGrad = 1, kEpiStore = 2 };
 
@@ -86,7 +87,7 @@ struct Params {
   // kEpiGrad
   const float* row_max;        // [rows], base 2
   const float* row_sum;
-  const float* grad;           // [rows], or NULL: 1 (a factor that all rows share is applied to the results)
+  const float* grad;           // factor per row of the column sums (kEpiGrad) or of the result (kEpiStore); NULL: 1
   float* bias_partials;        // [row blocks of 32][n_tiles * 256] or NULL
   __nv_bfloat16* d_out;        // [planes][panels of 64 columns][rows][64]
   int panels;                  // kEpiGrad: of d_out; kEpiStore: of A, which is such a matrix
@@ -246,12 +247,12 @@ __device__ __forceinline__ uint8_t* box_piece(uint8_t* box, int row, int piece) 
   return box + row * 64 + ((piece ^ ((row >> 1) & 3)) << 4);
 }
 // The box to memory, eight rows at a time, its columns added up in fp32 on the way (a lane moves four rows of eight
-// columns, the eight lanes of a column then share out the sums).  `out` is the box's first value; rows at and beyond
-// `rows` are not stored.  Returns the sums of columns box_column(lane) and the next, in both lanes of a pair 4 apart.
+// columns, each row times its lane's `factor`; the eight lanes of a column then share out the sums).  `out` is the box's
+// first value; rows at and beyond `rows` are not stored.  Returns the sums of columns box_column(lane) and the next, in both lanes of a pair 4 apart.
 // (A TMA store needs the whole group's barriers and a wait of 0.8 us until its buffer is free again.)
 __device__ __forceinline__ int box_column(int lane) { return (lane & 3) * 8 + ((lane >> 4) & 1) * 4 + ((lane >> 3) & 1) * 2; }
 template <bool SUMS>
-__device__ __forceinline__ float2 box_out(uint8_t* box, __nv_bfloat16* out, int ld, int rows, int lane) {
+__device__ __forceinline__ float2 box_out(uint8_t* box, __nv_bfloat16* out, int ld, int rows, int lane, float factor) {
   const int q = lane & 3, sub = lane >> 2;
   uint64_t acc[4] = {0ull, 0ull, 0ull, 0ull};
   __nv_bfloat16* dst = out + sub * ld + q * 8;
@@ -262,8 +263,10 @@ __device__ __forceinline__ float2 box_out(uint8_t* box, __nv_bfloat16* out, int 
     dst += 8 * ld;
     if (SUMS) {
       const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+      const float f = __shfl_sync(0xffffffffu, factor, 8 * r + sub);
+      const uint64_t f2 = pack2(f, f);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[e] = add2(acc[e], pack2(__uint_as_float(w[e] << 16), __uint_as_float(w[e] & 0xffff0000u)));
+      for (int e = 0; e < 4; ++e) acc[e] = fma2(pack2(__uint_as_float(w[e] << 16), __uint_as_float(w[e] & 0xffff0000u)), f2, acc[e]);
     }
   }
   float2 sums = make_float2(0.0f, 0.0f);
@@ -344,10 +347,10 @@ __device__ __forceinline__ void load_bias(const Params& p, float* dst, int64_t v
   }
 }
 
-// d = g * (2^(y - top) / sum - [target]) = coef * 2^(y - top) - [target] g; a row that does not count is all zero
+// d = 2^(y - top) / sum - [target]; a row that does not count is all zero
 struct RowTerms {
   int64_t target;              // word of the target relative to the first column, or -1
-  float top, coef, g;
+  float top, coef, g;          // coef = 1 / sum; g: the row's factor in the column sums
   bool counts;
 };
 __device__ __forceinline__ RowTerms row_terms(const Params& p, int64_t row, int64_t first_word) {
@@ -358,8 +361,8 @@ __device__ __forceinline__ RowTerms row_terms(const Params& p, int64_t row, int6
       if (t >= first_word) r.target = t - first_word;
       r.g = p.grad != nullptr ? __ldg(p.grad + row) : 1.0f;
       r.top = __ldg(p.row_max + row);
-      r.coef = r.g / __ldg(p.row_sum + row);
-      r.counts = r.coef != 0.0f || r.g != 0.0f;
+      r.coef = 1.0f / __ldg(p.row_sum + row);
+      r.counts = true;
     }
   }
   return r;
@@ -383,7 +386,7 @@ __device__ __forceinline__ void score_gradient(float (&y)[32], const float* bias
     const int at = hit ? static_cast<int>(r.target) - first : -1;
 #pragma unroll
     for (int j = 0; j < 32; ++j) {
-      if (at == j) y[j] -= r.g;
+      if (at == j) y[j] -= 1.0f;
     }
   }
 }
@@ -605,6 +608,14 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
       if (EPI == kEpiStore) {
         if (p.scale != nullptr) scale = *p.scale;
         if (p.scale2 != nullptr) scale *= *p.scale2;
+        if (p.grad != nullptr && live) {
+          // a row that does not count has d = 0 whatever its factor is; 0 x inf must not come of it
+          scale = __ldg(p.grad + row);
+          if (!isfinite(scale)) {
+            const int64_t t = __ldg(p.targets + row);
+            if (t == p.ignore_index || t < 0 || t >= p.vocab) scale = 0.0f;
+          }
+        }
       }
       int target_col = -1;                                   // kEpiLse: the target's column among this group's
       RowTerms terms{};
@@ -715,7 +726,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
           if (SEG && p.bias_partials != nullptr) {
             float v[32];
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = d[j];
+            for (int j = 0; j < 32; ++j) v[j] = d[j] * terms.g;
             col_sums[c + lane] = transpose_sum(v, lane);
           }
 #pragma unroll
@@ -740,10 +751,10 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
             __nv_bfloat16* dst = out + (c / 64) * panel + c % 64 + pl * (p.panels * panel);
             if (!SEG && p.bias_partials != nullptr) {
               // sums of the rounded values, which is what the weights' gradient is made of as well
-              const float2 sums = box_out<true>(box, dst, 64, rows_here, lane);
+              const float2 sums = box_out<true>(box, dst, 64, rows_here, lane, terms.g);
               if ((lane & 4) == 0) *reinterpret_cast<float2*>(col_sums + c + box_column(lane)) = sums;
             } else {
-              box_out<false>(box, dst, 64, rows_here, lane);
+              box_out<false>(box, dst, 64, rows_here, lane, 0.0f);
             }
             __syncwarp();
           }

@@ -28,7 +28,7 @@ def linear_cross_entropy(hidden: Tensor, weight: Tensor, targets: Tensor, bias: 
     "mean" (over the tokens that count; NaN if none does).  Tokens with ``target == ignore_index`` have loss 0 and
     a zero gradient.  Any other target outside the vocabulary is ignored too and reported by
     ``cuda_ops.check_device_errors``.  A word whose bias is ``-inf`` is masked: it has probability 0.
-    The hidden states of ignored tokens must be finite (they are multiplied by a zero gradient).
+    What the hidden states of ignored tokens hold, NaN included, reaches neither loss nor gradients.
     """
     cuda_ops._require_extension("linear_cross_entropy")
     if reduction not in _REDUCTIONS:

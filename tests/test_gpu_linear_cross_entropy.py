@@ -5,7 +5,8 @@ fp32 step (2^-23, also if it truncates), so |error of y_ij| <= e_ij = (D + 16) 2
 plane products of full precision lose at most 3 x 2^-24 of each product on top, which the 16 covers at D >= 1 with
 the joins and the base-2 scaling.  With e_i = max_j e_ij the loss is off by at most 2 e_i plus a few steps of the
 logarithm; a probability by a factor of exp(2 e_i + 2^-20) (the exponential's own error is below 2^-21).  d = p - [target] is rounded
-once to bf16 (2^-8 of itself; in full precision 2^-24, three planes) before it is multiplied, the products accumulate as
+once to bf16 (2^-8 of itself; in full precision 2^-24, three planes) before it is multiplied; with a factor per token the
+tokens that dW multiplies it with are rounded once more, x g to the same type; the products accumulate as
 above -- over at most 128 + 8 additions between two roundings in full precision, over the whole contraction in
 bf16 -- and the result is rounded once to its own type.
 """
@@ -59,7 +60,8 @@ def reference(x, w, b, t, upstream, ignore_index=-100):
     for name, a, a_tol, other, length in (("x", d, d_tol, W, len(W)), ("w", d.T, d_tol.T, X, len(X))):
         grads[name] = a @ other
         steps = 136 + length * 6 / (64 * 32) if dtype == torch.float32 else length + 16
-        tols[name] = (a_tol + steps * 2.0 ** -23 * a.abs()) @ other.abs() + 2 * HALF_STEP[dtype] * grads[name].abs()
+        weighted = HALF_STEP[dtype] if name == "w" and not torch.equal(upstream, upstream[:1].expand_as(upstream)) else 0.0
+        tols[name] = (a_tol + (steps * 2.0 ** -23 + weighted) * a.abs()) @ other.abs() + 2 * HALF_STEP[dtype] * grads[name].abs()
     if b is not None:
         grads["b"] = d.sum(0)
         # sums of the same rounded d, in fp32 additions, 32 rows and then the blocks
@@ -229,6 +231,29 @@ def test_values_that_are_not_finite_stay_in_their_rows():
     assert torch.isnan(loss[[1, 4]]).all() and torch.equal(loss[[0, 2, 3, 5]], clean[[0, 2, 3, 5]])
     closed = torch.full((300,), float("-inf"), device=DEV)
     assert torch.isnan(linear_cross_entropy(x, w, t, closed, reduction="none")).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("reduction", ["none", "mean"])
+def test_what_ignored_tokens_hold_goes_nowhere(dtype, reduction):
+    x, w, b, t = make(300, 72, 513, dtype, dtype, ignored=0.3, seed=18)
+    up = torch.rand(300, device=DEV) if reduction == "none" else None
+
+    def step(x, up):
+        x = x.clone().requires_grad_(True)
+        leaves = [x, w.clone().requires_grad_(True), b.clone().requires_grad_(True)]
+        loss = linear_cross_entropy(leaves[0], leaves[1], t, leaves[2], reduction=reduction)
+        return (loss.detach(), *torch.autograd.grad(loss, leaves, up))
+
+    clean = step(x, up)
+    bad, skip = x.clone(), (t == -100).nonzero()[:, 0]
+    bad[skip[0]] = float("nan")
+    bad[skip[1], 3] = float("inf")
+    if up is not None:
+        up = up.clone()
+        up[skip[2]], up[skip[3]] = float("inf"), float("nan")
+    for p, q in zip(clean, step(bad, up)):
+        assert torch.equal(p, q)
 
 
 def test_large_scores_and_a_certain_target():
