@@ -433,11 +433,12 @@ int grmx_archive_push(const float* memory, float* archive, void* archive_bf16, i
  * sum of the scores' exponentials, base 2) and inv_count float32 [1] are what the backward call needs.
  * bf16 products are exact and accumulate in fp32; fp32 inputs are split into three bf16 parts each, of which
  * the six products above 2^-24 are taken.  Masked words (bias -inf) have probability 0; a row without any
- * finite score gives NaN, as does a score of +inf or NaN.
+ * finite score gives NaN, as does a score of +inf or NaN.  What a token that does not count holds in hidden,
+ * NaN included, reaches neither loss nor gradients.
  *
  * workspace: device memory of grmx_linear_xent_workspace(N, D, V, dtype, backward) bytes (0 if N == 0, -1 for
- * sizes or a dtype that are refused), 256-byte aligned, contents irrelevant, not shared between calls that may
- * run at the same time.
+ * sizes or a dtype that are refused; the current device's number of SMs goes into it), 256-byte aligned,
+ * contents irrelevant, not shared between calls that may run at the same time.
  *
  * The reference computes this as output_layer (grm/utils/train.py:223) followed by torch's cross entropy.
  */

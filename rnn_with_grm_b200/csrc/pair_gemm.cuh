@@ -6,8 +6,12 @@
 // 64-wide k block), and its own 128 rows of the result in TMEM: a pair reads (256 + 256) * 64 values per
 // 2 * 256 * 256 * 64 FLOP, half of what a single CTA with a 128 x 256 tile would ask of L2 for its share,
 // which is what decides whether the tensor cores are fed.  Persistent pairs; one warp loads (TMA ring of
-// kStages blocks), one warp of the first CTA issues for both, the others are the epilogue in groups of four.  Two accumulators
-// of 256 columns: the epilogue of a tile runs under the products of the next one.
+// kStages blocks), one warp of the first CTA issues for both, the others are the epilogue in groups of four.  Two
+// accumulators of 256 columns: the epilogue of a tile runs under the products of the next one.
+//
+// Measured and dropped: B resident in shared memory while a pair walks down its rows (contractions of at most 512: no
+// gain once the card is at its power limit); an epilogue that stores by TMA from a buffer per group (594 us where a
+// staging box per warp and plain stores take 536).
 //
 // The gradient of the scores goes out, and comes back as A of the products that follow, in panels of 64 columns
 // [rows][64]: a tile's part is then whole kilobytes in a row, where lines of a wide row-major matrix would be 64 KiB
@@ -72,7 +76,6 @@ struct Params {
   int m_tiles, n_tiles, splits;
   int k_blocks;                // 64-wide blocks of the contraction
   int blocks_per_split;
-  int products;                // 1, or 6 plane products per block
   int64_t rows, cols;          // true size of the result
   // loss epilogues: columns are words v0 + n of the vocabulary
   int64_t v0, vocab;
