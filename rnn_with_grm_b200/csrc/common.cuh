@@ -31,6 +31,29 @@ uint32_t* device_error_word_ptr();
     if (!(cond)) return ::grmx::fail(GRMX_ERR_ARG, __VA_ARGS__); \
   } while (0)
 
+// ---- kernels that follow each other closely ----
+// The next kernel of the stream may be set up while this one still runs (and does so if it was launched by launch_after);
+// it waits in wait_for_previous() until everything before it has completed.  Every kernel launched by launch_after calls
+// that before it touches memory.
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <typename... Params, typename... Args>
+inline void launch_after(void (*kernel)(Params...), unsigned grid_x, unsigned grid_y, int threads, int smem, cudaStream_t stream,
+                         Args... args) {
+  cudaLaunchAttribute attribute = {};
+  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(grid_x, grid_y, 1);
+  config.blockDim = dim3(threads, 1, 1);
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  cudaLaunchKernelEx(&config, kernel, static_cast<Params>(args)...);      // its error is picked up by check_launch
+}
+
 // ---- element conversion ----
 template <typename T>
 __device__ __forceinline__ float to_float(T v);

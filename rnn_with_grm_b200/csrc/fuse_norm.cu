@@ -347,6 +347,8 @@ fuse_norm_fwd_kernel(const __grid_constant__ RowArgs a) {
   constexpr int kGroups = threads_of(G) / G;
   __shared__ float2 s_scratch[kGroups][2][G / 32];
   int turn = 0;
+  let_next_start();
+  wait_for_previous();
   extern __shared__ float s_params[];                    // shifted rows: weight, bias, scale
   const int group = threadIdx.x / G, lane = threadIdx.x % G;
   const int H = a.H;
@@ -451,6 +453,8 @@ fuse_norm_bwd_kernel(const __grid_constant__ RowArgs a) {
   constexpr int kGroups = threads_of(G) / G;
   __shared__ float2 s_scratch[kGroups][2][G / 32];
   int turn = 0;
+  let_next_start();
+  wait_for_previous();
   extern __shared__ float s_dynamic[];                   // shifted rows: weight, scale; then, at the end, the column sums
   const int group = threadIdx.x / G, lane = threadIdx.x % G;
   const int H = a.H;
@@ -645,6 +649,8 @@ template <typename P>
 __global__ void __launch_bounds__(1024) fuse_norm_cols_kernel(const float* __restrict__ partials, int ctas, int H, P* out0, P* out1,
                                                               P* out2) {
   __shared__ float s_sum[32][33];
+  let_next_start();
+  wait_for_previous();
   const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
   const int h = blockIdx.x * 32 + lane;
   const float* src = partials + static_cast<int64_t>(blockIdx.y) * ctas * H;
@@ -705,7 +711,7 @@ int launch_rows(Kernel kernel, const RowArgs& a, int64_t grid, int threads, int 
   if (smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
     return fail(GRMX_ERR_LAUNCH, "%s: cannot reserve %d bytes of shared memory: %s", what, smem, cudaGetErrorString(cudaGetLastError()));
   }
-  kernel<<<static_cast<unsigned>(grid), threads, smem, s>>>(a);
+  launch_after(kernel, static_cast<unsigned>(grid), 1, threads, smem, s, a);
   return check_launch(what);
 }
 
@@ -870,10 +876,10 @@ extern "C" int grmx_fuse_norm_bwd(const void* grad_out, const void* grad_sum, co
   }
   const dim3 grid(static_cast<unsigned>((H + 31) / 32), static_cast<unsigned>(kinds));
   if (param_dtype == GRMX_F32) {
-    fuse_norm_cols_kernel<float><<<grid, 1024, 0, s>>>(a.col_partials, static_cast<int>(ctas), a.H, static_cast<float*>(outs[0]),
+    launch_after(fuse_norm_cols_kernel<float>, grid.x, grid.y, 1024, 0, s, a.col_partials, static_cast<int>(ctas), a.H, static_cast<float*>(outs[0]),
                                                        static_cast<float*>(outs[1]), static_cast<float*>(outs[2]));
   } else {
-    fuse_norm_cols_kernel<__nv_bfloat16><<<grid, 1024, 0, s>>>(
+    launch_after(fuse_norm_cols_kernel<__nv_bfloat16>, grid.x, grid.y, 1024, 0, s, 
         a.col_partials, static_cast<int>(ctas), a.H, static_cast<__nv_bfloat16*>(outs[0]), static_cast<__nv_bfloat16*>(outs[1]),
         static_cast<__nv_bfloat16*>(outs[2]));
   }

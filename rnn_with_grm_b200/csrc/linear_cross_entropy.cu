@@ -47,6 +47,8 @@ struct TokenRows {
 template <typename T, int PLANES>
 __global__ void __launch_bounds__(256) planes_kernel(const T* __restrict__ src, __nv_bfloat16* __restrict__ dst, int64_t rows,
                                                      int cols, int ld, int64_t plane_stride, TokenRows tokens) {
+  let_next_start();
+  wait_for_previous();
   const int64_t pairs = ld / 2;
   const int64_t total = rows * pairs;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * 256) {
@@ -102,10 +104,10 @@ int copy_operand(Operand* out, const void* src, int64_t rows, int64_t cols, int 
   const unsigned grid = static_cast<unsigned>(blocks < 148 * 16 ? blocks : 148 * 16);
   __nv_bfloat16* d = reinterpret_cast<__nv_bfloat16*>(dst);
   if (dtype == GRMX_F32) {
-    planes_kernel<float, 3><<<grid, 256, 0, s>>>(static_cast<const float*>(src), d, rows, static_cast<int>(cols),
+    launch_after(planes_kernel<float, 3>, grid, 1, 256, 0, s, static_cast<const float*>(src), d, rows, static_cast<int>(cols),
                                                   static_cast<int>(ld), stride, tokens);
   } else {
-    planes_kernel<__nv_bfloat16, 1><<<grid, 256, 0, s>>>(static_cast<const __nv_bfloat16*>(src), d, rows,
+    launch_after(planes_kernel<__nv_bfloat16, 1>, grid, 1, 256, 0, s, static_cast<const __nv_bfloat16*>(src), d, rows,
                                                           static_cast<int>(cols), static_cast<int>(ld), stride, tokens);
   }
   *out = Operand{dst, ld, stride, planes};
@@ -207,6 +209,8 @@ few_tokens_kernel(const T* __restrict__ hidden, const T* __restrict__ weight, co
       for (int h = 0; h < 2; ++h) raw[r][h] = load_features(row, d0 + (h * 32 + lane) * G, D, aligned != 0);
     }
   };
+  let_next_start();
+  wait_for_previous();
   load(v0, 0);                                             // on its way while the tokens are staged
   if (blockIdx.x == 0 && threadIdx.x == 0) *ticket = 0u;
   for (int i = threadIdx.x; i < TOKENS * pitch; i += kFewThreads) {
@@ -298,7 +302,7 @@ int launch_few_tokens(const void* hidden, const void* weight, const void* bias, 
   if (smem > 40 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
     return fail(GRMX_ERR_LAUNCH, "loss of a few tokens: cannot reserve %d bytes of shared memory: %s", smem, cudaGetErrorString(cudaGetLastError()));
   }
-  kernel<<<few_tokens_blocks(V), kFewThreads, smem, s>>>(static_cast<const T*>(hidden), static_cast<const T*>(weight), bias, bias_dtype,
+  launch_after(kernel, few_tokens_blocks(V), 1, kFewThreads, smem, s, static_cast<const T*>(hidden), static_cast<const T*>(weight), bias, bias_dtype,
                                                          targets, ignore_index, tokens, D, V, aligned, partials, target_score, ticket);
   return check_launch("loss of a few tokens");
 }
@@ -324,6 +328,8 @@ loss_join_kernel(const float2* __restrict__ partials, const float* __restrict__ 
   __shared__ double s_loss[kJoinThreads];
   __shared__ int s_count[kJoinThreads];
   __shared__ bool s_last;
+  let_next_start();
+  wait_for_previous();
   const int r = threadIdx.x % ROWS, slice = threadIdx.x / ROWS;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + r;
   float2 all = make_float2(-INFINITY, 0.0f);
@@ -417,6 +423,8 @@ int join_rows(int64_t N) { return N >= 16384 ? 32 : N >= 512 ? 8 : 1; }
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256) sum_splits_kernel(const float* __restrict__ part, T* __restrict__ out, int64_t rows,
                                                          int cols, int ld, int64_t split_stride, int splits) {
+  let_next_start();
+  wait_for_previous();
   const int per_row = cols / VEC;
   const int64_t total = rows * per_row;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * 256) {
@@ -452,12 +460,12 @@ int launch_sum_splits(const float* part, void* out, int64_t rows, int64_t cols, 
   const unsigned grid = static_cast<unsigned>(blocks < 148 * 16 ? blocks : 148 * 16);
   const int c = static_cast<int>(cols), l = static_cast<int>(ld);
   if (dtype == GRMX_F32) {
-    if (vec) sum_splits_kernel<float, 4><<<grid, 256, 0, s>>>(part, static_cast<float*>(out), rows, c, l, split_stride, splits);
-    else sum_splits_kernel<float, 1><<<grid, 256, 0, s>>>(part, static_cast<float*>(out), rows, c, l, split_stride, splits);
+    if (vec) launch_after(sum_splits_kernel<float, 4>, grid, 1, 256, 0, s, part, static_cast<float*>(out), rows, c, l, split_stride, splits);
+    else launch_after(sum_splits_kernel<float, 1>, grid, 1, 256, 0, s, part, static_cast<float*>(out), rows, c, l, split_stride, splits);
   } else {
     __nv_bfloat16* o = static_cast<__nv_bfloat16*>(out);
-    if (vec) sum_splits_kernel<__nv_bfloat16, 4><<<grid, 256, 0, s>>>(part, o, rows, c, l, split_stride, splits);
-    else sum_splits_kernel<__nv_bfloat16, 1><<<grid, 256, 0, s>>>(part, o, rows, c, l, split_stride, splits);
+    if (vec) launch_after(sum_splits_kernel<__nv_bfloat16, 4>, grid, 1, 256, 0, s, part, o, rows, c, l, split_stride, splits);
+    else launch_after(sum_splits_kernel<__nv_bfloat16, 1>, grid, 1, 256, 0, s, part, o, rows, c, l, split_stride, splits);
   }
   return check_launch("loss split sums");
 }
@@ -468,6 +476,8 @@ __global__ void __launch_bounds__(256) bias_sum_kernel(const float* __restrict__
                                                        int64_t cols, const float* scale, const float* scale2,
                                                        T* __restrict__ out) {
   __shared__ float s_sum[8][32];
+  let_next_start();
+  wait_for_previous();
   const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
   const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;
   float sum = 0.0f;
@@ -519,7 +529,7 @@ int launch_pair(const Maps& maps, const Params& p, const char* what, cudaStream_
   const int64_t units = static_cast<int64_t>(p.m_tiles) * p.n_tiles * p.splits;
   const int pairs = pairs_on_device();
   const unsigned grid = 2u * static_cast<unsigned>(units < pairs ? units : pairs);
-  kernel<<<grid, threads_of(EPI, SEG), kSmemAlloc, s>>>(maps, p, device_error_word_ptr());
+  launch_after(kernel, grid, 1, threads_of(EPI, SEG), kSmemAlloc, s, maps, p, device_error_word_ptr());
   return check_launch(what);
 }
 
@@ -713,8 +723,8 @@ extern "C" int grmx_linear_xent_fwd(const void* hidden, const void* weight, cons
     GRMX_TRY(launch_scores<kEpiLse>(maps, p, dtype, "loss scores", s));
   }
   auto join_kernel = join_rows(N) == 32 ? loss_join_kernel<32> : join_rows(N) == 8 ? loss_join_kernel<8> : loss_join_kernel<1>;
-  join_kernel<<<static_cast<unsigned>(f.join_blocks), kJoinThreads, 0, s>>>(
-      partials, target_score, targets, ignore_index, V, N, f.parts, reduction, row_stats, row_stats + N, loss, inv_count,
+  launch_after(
+      join_kernel, static_cast<unsigned>(f.join_blocks), 1, kJoinThreads, 0, s, partials, target_score, targets, ignore_index, V, N, f.parts, reduction, row_stats, row_stats + N, loss, inv_count,
       reinterpret_cast<double*>(ws + f.off_loss), reinterpret_cast<int*>(ws + f.off_count), ticket, device_error_word_ptr());
   return check_launch("loss join");
 }
@@ -810,9 +820,9 @@ extern "C" int grmx_linear_xent_bwd(const float* grad_loss, const void* hidden, 
       const int64_t blocks = ceil_div(N, kTileM) * 8;
       const unsigned grid = static_cast<unsigned>(ceil_div(words, 32));
       if (bias_dtype == GRMX_F32) {
-        bias_sum_kernel<float><<<grid, 256, 0, s>>>(part_b, blocks, width, words, scale, scale2, static_cast<float*>(grad_bias) + v0);
+        launch_after(bias_sum_kernel<float>, grid, 1, 256, 0, s, part_b, blocks, width, words, scale, scale2, static_cast<float*>(grad_bias) + v0);
       } else {
-        bias_sum_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(part_b, blocks, width, words, scale, scale2,
+        launch_after(bias_sum_kernel<__nv_bfloat16>, grid, 1, 256, 0, s, part_b, blocks, width, words, scale, scale2,
                                                              static_cast<__nv_bfloat16*>(grad_bias) + v0);
       }
       GRMX_TRY(check_launch("loss bias gradient"));

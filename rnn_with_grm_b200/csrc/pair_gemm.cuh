@@ -435,7 +435,6 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
     *s_abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (EPI == kEpiLse && blockIdx.x == 0 && tid == 0 && p.ticket != nullptr) *p.ticket = 0u;
   if (warp == kIssuerWarp) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(s_tmem)), "r"(512u)
                  : "memory");
@@ -447,6 +446,9 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
   cluster_sync();
   tc_fence_after();
   const uint32_t tmem_base = *s_tmem;
+  let_next_start();
+  wait_for_previous();                  // nothing above touches memory
+  if (EPI == kEpiLse && blockIdx.x == 0 && tid == 0 && p.ticket != nullptr) *p.ticket = 0u;
 
   const Units<EPI> units(p);
   auto split_range = [&](int s, int& k0, int& k1) {
