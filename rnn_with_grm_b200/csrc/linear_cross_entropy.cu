@@ -755,7 +755,6 @@ extern "C" int grmx_linear_xent_bwd(const float* grad_loss, const void* hidden, 
   const int planes = f32 ? 3 : 1;
   const int64_t elem = f32 ? 4 : 2;
   Operand x, w;
-  GRMX_TRY(make_operand(&x, hidden, N, D, dtype, ws + b.off_x, s));
   GRMX_TRY(make_operand(&w, weight, V, D, dtype, ws + b.off_w, s));
   const int n_tiles_d = static_cast<int>(ceil_div(D, kTileN));
   float* part_x = reinterpret_cast<float*>(ws + b.off_dx);
@@ -771,6 +770,11 @@ extern "C" int grmx_linear_xent_bwd(const float* grad_loss, const void* hidden, 
   Operand x_counted;
   if (grad_weight != nullptr) {
     GRMX_TRY(copy_operand(&x_counted, hidden, N, D, dtype, ws + b.off_xc, TokenRows{targets, ignore_index, V, per_row ? grad_loss : nullptr}, s));
+  }
+  if (grad_weight != nullptr && !per_row && !readable_in_place(hidden, D, dtype)) {
+    x = x_counted;             // the scores of tokens that do not count are not looked at
+  } else {
+    GRMX_TRY(make_operand(&x, hidden, N, D, dtype, ws + b.off_x, s));
   }
   // a result that is complete after one product leaves its epilogue in the caller's type
   auto storable = [&](const void* out) { return D * elem % 16 == 0 && (reinterpret_cast<uintptr_t>(out) & 15u) == 0; };
