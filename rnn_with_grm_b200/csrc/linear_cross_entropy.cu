@@ -11,7 +11,7 @@
 //
 // Bound by the tensor cores at training sizes, by the stream of W where a few tokens are scored.  16384 tokens x 512
 // x 32768 words, bf16, cool / back to back (then the card is at its power limit): scores and their maxima 350 / 400 us
-// (1.57 PFLOP/s cool, 0.95 of cuBLAS's burst), gradient of the scores 521 / 584, dx 355 / 450, dW 365 / 465.  The gradient
+// (1.57 PFLOP/s cool, 0.95 of cuBLAS's burst), gradient of the scores 519 / 595, dx 355 / 450, dW 375 / 475.  The gradient
 // kernel is bound by its epilogue: 110 us of it go when nothing is stored (1 GB), 30 each for exponentials and column sums.
 // The maximum and the sum are kept apart (never as one log-sum-exp): exp(y - max) / sum then carries no
 // rounding of a sum that is as large as the scores, and a target that is the maximum itself leaves exactly
@@ -508,9 +508,9 @@ int pairs_on_device() {
   return cached[device];
 }
 
-template <int EPI, bool A_MN, bool B_MN, bool SEG>
+template <int EPI, bool A_MN, bool B_MN, bool SEG, bool WEIGHTED = false>
 int launch_pair(const Maps& maps, const Params& p, const char* what, cudaStream_t s) {
-  auto kernel = pair_gemm_kernel<EPI, A_MN, B_MN, SEG>;
+  auto kernel = pair_gemm_kernel<EPI, A_MN, B_MN, SEG, WEIGHTED>;
   static std::mutex mutex;
   static bool configured[64] = {false};
   int device = 0;
@@ -536,6 +536,10 @@ int launch_pair(const Maps& maps, const Params& p, const char* what, cudaStream_
 // the products whose epilogue works on scores
 template <int EPI>
 int launch_scores(const Maps& maps, const Params& p, int dtype, const char* what, cudaStream_t s) {
+  if (EPI == kEpiGrad && p.grad != nullptr) {
+    return dtype == GRMX_F32 ? launch_pair<EPI, false, false, true, EPI == kEpiGrad>(maps, p, what, s)
+                             : launch_pair<EPI, false, false, false, EPI == kEpiGrad>(maps, p, what, s);
+  }
   if (dtype == GRMX_F32) return launch_pair<EPI, false, false, true>(maps, p, what, s);
   return launch_pair<EPI, false, false, false>(maps, p, what, s);
 }

@@ -250,11 +250,11 @@ __device__ __forceinline__ uint8_t* box_piece(uint8_t* box, int row, int piece) 
   return box + row * 64 + ((piece ^ ((row >> 1) & 3)) << 4);
 }
 // The box to memory, eight rows at a time, its columns added up in fp32 on the way (a lane moves four rows of eight
-// columns, each row times its lane's `factor`; the eight lanes of a column then share out the sums).  `out` is the box's
+// columns, each row times its lane's `factor` if WEIGHTED; the eight lanes of a column then share out the sums).  `out` is the box's
 // first value; rows at and beyond `rows` are not stored.  Returns the sums of columns box_column(lane) and the next, in both lanes of a pair 4 apart.
 // (A TMA store needs the whole group's barriers and a wait of 0.8 us until its buffer is free again.)
 __device__ __forceinline__ int box_column(int lane) { return (lane & 3) * 8 + ((lane >> 4) & 1) * 4 + ((lane >> 3) & 1) * 2; }
-template <bool SUMS>
+template <bool SUMS, bool WEIGHTED = false>
 __device__ __forceinline__ float2 box_out(uint8_t* box, __nv_bfloat16* out, int ld, int rows, int lane, float factor) {
   const int q = lane & 3, sub = lane >> 2;
   uint64_t acc[4] = {0ull, 0ull, 0ull, 0ull};
@@ -266,10 +266,13 @@ __device__ __forceinline__ float2 box_out(uint8_t* box, __nv_bfloat16* out, int 
     dst += 8 * ld;
     if (SUMS) {
       const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-      const float f = __shfl_sync(0xffffffffu, factor, 8 * r + sub);
+      const float f = WEIGHTED ? __shfl_sync(0xffffffffu, factor, 8 * r + sub) : 1.0f;
       const uint64_t f2 = pack2(f, f);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[e] = fma2(pack2(__uint_as_float(w[e] << 16), __uint_as_float(w[e] & 0xffff0000u)), f2, acc[e]);
+      for (int e = 0; e < 4; ++e) {
+        const uint64_t pair = pack2(__uint_as_float(w[e] << 16), __uint_as_float(w[e] & 0xffff0000u));
+        acc[e] = WEIGHTED ? fma2(pair, f2, acc[e]) : add2(acc[e], pair);
+      }
     }
   }
   float2 sums = make_float2(0.0f, 0.0f);
@@ -356,13 +359,14 @@ struct RowTerms {
   float top, coef, g;          // coef = 1 / sum; g: the row's factor in the column sums
   bool counts;
 };
+template <bool WEIGHTED>
 __device__ __forceinline__ RowTerms row_terms(const Params& p, int64_t row, int64_t first_word) {
   RowTerms r{-1, 0.0f, 0.0f, 0.0f, false};
   if (row < p.rows) {
     const int64_t t = __ldg(p.targets + row);
     if (t != p.ignore_index && t >= 0 && t < p.vocab) {
       if (t >= first_word) r.target = t - first_word;
-      r.g = p.grad != nullptr ? __ldg(p.grad + row) : 1.0f;
+      if (WEIGHTED) r.g = __ldg(p.grad + row);
       r.top = __ldg(p.row_max + row);
       r.coef = 1.0f / __ldg(p.row_sum + row);
       r.counts = true;
@@ -396,7 +400,9 @@ __device__ __forceinline__ void score_gradient(float (&y)[32], const float* bias
 
 // SEG: full precision (six plane products, accumulator drained into registers; both epilogue groups work on
 // every tile).  Otherwise half of the groups work on each accumulator, so on every other tile.
-template <int EPI, bool A_MN, bool B_MN, bool SEG>
+// WEIGHTED (kEpiGrad): the column sums have a factor per row; a kernel of its own, since the plain one is slower by 25 us of
+// 525 with both in it.
+template <int EPI, bool A_MN, bool B_MN, bool SEG, bool WEIGHTED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(EPI, SEG), 1)
 pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p, uint32_t* error_word) {
   constexpr int kGroups = groups_of(EPI, SEG);
@@ -446,7 +452,6 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
   cluster_sync();
   tc_fence_after();
   const uint32_t tmem_base = *s_tmem;
-  let_next_start();
   wait_for_previous();                  // nothing above touches memory
   if (EPI == kEpiLse && blockIdx.x == 0 && tid == 0 && p.ticket != nullptr) *p.ticket = 0u;
 
@@ -628,7 +633,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
         group_sync(bar_id);                                  // everyone is done with the previous tile's s_bias
         const int64_t first_word = p.v0 + static_cast<int64_t>(n) * kTileN + c0;
         load_bias(p, s_bias, first_word, kCols, gt, kGroupThreads);
-        if (EPI == kEpiGrad) terms = row_terms(p, row, first_word);
+        if (EPI == kEpiGrad) terms = row_terms<WEIGHTED>(p, row, first_word);
         if (EPI == kEpiLse && live) {
           const int64_t rel = __ldg(p.targets + row) - first_word;
           if (rel >= 0 && rel < kCols && __ldg(p.targets + row) != p.ignore_index) target_col = static_cast<int>(rel);
@@ -731,7 +736,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
           if (SEG && p.bias_partials != nullptr) {
             float v[32];
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = d[j] * terms.g;
+            for (int j = 0; j < 32; ++j) v[j] = WEIGHTED ? d[j] * terms.g : d[j];
             col_sums[c + lane] = transpose_sum(v, lane);
           }
 #pragma unroll
@@ -756,7 +761,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
             __nv_bfloat16* dst = out + (c / 64) * panel + c % 64 + pl * (p.panels * panel);
             if (!SEG && p.bias_partials != nullptr) {
               // sums of the rounded values, which is what the weights' gradient is made of as well
-              const float2 sums = box_out<true>(box, dst, 64, rows_here, lane, terms.g);
+              const float2 sums = box_out<true, WEIGHTED>(box, dst, 64, rows_here, lane, terms.g);
               if ((lane & 4) == 0) *reinterpret_cast<float2*>(col_sums + c + box_column(lane)) = sums;
             } else {
               box_out<false>(box, dst, 64, rows_here, lane, 0.0f);
@@ -808,6 +813,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
     if (gt == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
 
+  let_next_start();                     // (at the start it costs the products 2 %)
   tc_fence_before();
   __syncthreads();
   if (tid == 0 && *s_abort && error_word != nullptr) atomicOr(error_word, kErrBoundedWait);
