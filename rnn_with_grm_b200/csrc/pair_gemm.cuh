@@ -594,9 +594,9 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
     auto box_end = [&](int x, int y, int z, bool add) {
       fence_proxy_async();
       group_sync(bar_id);
-      if (gt == 0 && y < p.rows) {                           // a box wholly below the matrix is not sent
-        store_box(stage + (boxes % kBuffers) * kStoreBytes, &maps.c, x, y, z, add);
-        bulk_commit();
+      if (gt == 0) {
+        if (y < p.rows) store_box(stage + (boxes % kBuffers) * kStoreBytes, &maps.c, x, y, z, add);
+        bulk_commit();       // a box wholly below the matrix is an empty group: box_begin counts groups as boxes
       }
       ++boxes;
     };
