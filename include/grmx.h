@@ -471,8 +471,8 @@ int grmx_linear_xent_bwd(const float* grad_loss, const void* hidden, const void*
  *
  * online, update, gate, out, sum_out [rows,H] in `dtype` (GRMX_F32 or GRMX_BF16); scale, ln_weight, ln_bias [H]
  * in param_dtype (GRMX_F32, or dtype), each NULL for the identity; sum_out (s itself, rounded once) may be NULL.
- * row_stats float32 [rows,2] (mean and rstd, what the backward call needs) may be NULL.  H <= 8192; arithmetic in
- * fp32.  Rows and parameters on 16-byte boundaries move in 16-byte pieces, others value by value.
+ * row_stats float32 [rows,2] (mean and rstd, what the backward call needs), 8-byte aligned, may be NULL.
+ * H <= 8192; arithmetic in fp32.  Rows and parameters on 16-byte boundaries move in 16-byte pieces, others value by value.
  * out may not overlap the inputs.
  *
  * Replaces the residual and gate rules of RetrievedStateFusion with its LayerNorm (grm/core/aggregator.py:116-145)

@@ -792,6 +792,7 @@ extern "C" int grmx_fuse_norm_fwd(const void* online, const void* update, const 
   if (rc != GRMX_OK) return rc;
   if (rows == 0) return GRMX_OK;
   GRMX_REQUIRE(online && update && out, "%s: NULL tensor pointer", who);
+  GRMX_REQUIRE((reinterpret_cast<uintptr_t>(row_stats) & 7u) == 0, "%s: row_stats must be 8-byte aligned", who);
   RowArgs a = {};
   a.online = online;
   a.update = update;
@@ -838,6 +839,7 @@ extern "C" int grmx_fuse_norm_bwd(const void* grad_out, const void* grad_sum, co
     return GRMX_OK;
   }
   GRMX_REQUIRE(online && update && row_stats, "%s: NULL tensor pointer", who);
+  GRMX_REQUIRE((reinterpret_cast<uintptr_t>(row_stats) & 7u) == 0, "%s: row_stats must be 8-byte aligned", who);
   GRMX_REQUIRE(grad_out || grad_sum, "%s: neither output has a gradient", who);
   const int kinds = (grad_weight != nullptr) + (grad_bias != nullptr) + (grad_scale != nullptr);
   RowArgs a = {};

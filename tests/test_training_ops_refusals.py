@@ -93,3 +93,13 @@ def test_language_model_loss_checks_its_arguments(lib):
     body = {k[len("grm_rnn."):]: torch.zeros(s) for k, s in shapes.items() if k.startswith("grm_rnn.")}
     with pytest.raises(ValueError, match="language"):
         StackedSegmentMemoryRunner(body, 1, **kwargs).loss(ids, ids)
+
+
+def test_fuse_norm_refuses_row_statistics_off_their_pairs(lib):
+    some, tail = 256, (4, 64, cabi.F32, cabi.F32)
+    for off in (260, 258, 257):
+        assert lib.grmx_fuse_norm_fwd(some, some, None, None, None, None, 1e-5, some, None, off, *tail, None) == 1
+        assert b"row_stats must be 8-byte aligned" in lib.grmx_last_error()
+        assert lib.grmx_fuse_norm_bwd(some, None, some, some, None, None, None, off, some, some, None, None, None, None, *tail,
+                                      None, 0, None) == 1
+        assert b"row_stats must be 8-byte aligned" in lib.grmx_last_error()
