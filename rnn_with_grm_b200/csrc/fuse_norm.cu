@@ -708,7 +708,8 @@ int64_t most_backward_ctas(int64_t rows, int64_t H) {
 
 template <typename Kernel>
 int launch_rows(Kernel kernel, const RowArgs& a, int64_t grid, int threads, int smem, const char* what, cudaStream_t s) {
-  if (smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
+  // (48 KiB without being asked for, less what the kernel holds itself: up to 512 bytes)
+  if (smem > 40 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
     return fail(GRMX_ERR_LAUNCH, "%s: cannot reserve %d bytes of shared memory: %s", what, smem, cudaGetErrorString(cudaGetLastError()));
   }
   launch_after(kernel, static_cast<unsigned>(grid), 1, threads, smem, s, a);

@@ -276,3 +276,11 @@ def test_rows_behind_the_last_stay_as_they_are():
                                       cabi.current_stream()))
     torch.cuda.synchronize()
     assert torch.equal(out[:5], call(t)) and (out[5:] == 7.0).all()
+
+
+# rows that are not a multiple of 16 bytes keep their parameters in shared memory: widths where these and the rows' own
+# few hundred bytes meet 48 KiB, forward (three vectors) and backward (two)
+@pytest.mark.parametrize("H", [3630, 3631, 3635, 3637, 3639, 3641, 5401, 5405, 5433, 5459, 5461, 5463])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+def test_parameters_of_about_48_kib(dtype, H):
+    check(make(5, H, dtype, True, True, seed=H), with_sum=True)
