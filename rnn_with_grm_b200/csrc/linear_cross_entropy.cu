@@ -137,6 +137,7 @@ __device__ __forceinline__ float2 join(float2 a, float2 b) {
 // One token, 512 x 32768 bf16: 21 us as a padded tile of the product, 11.5 us so (2.9 TB/s, half of it latency).
 constexpr int kFewTokens = 8;
 constexpr int kFewThreads = 256;
+constexpr int kFewShared = 160 * 1024;       // most shared memory for the tokens' features
 
 // sum of each of M values over the lanes; lane l returns that of value l / (32 / M)
 template <int M>
@@ -299,8 +300,9 @@ int launch_few_tokens(const void* hidden, const void* weight, const void* bias, 
                 : padded == 2 ? few_tokens_kernel<T, 2, kFewRows>
                 : padded == 4 ? few_tokens_kernel<T, 4, kFewRows>
                               : few_tokens_kernel<T, 8, 4>;
-  if (smem > 40 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
-    return fail(GRMX_ERR_LAUNCH, "loss of a few tokens: cannot reserve %d bytes of shared memory: %s", smem, cudaGetErrorString(cudaGetLastError()));
+  // always the same size: a limit of this call's own could be lowered by another thread's call before the launch below
+  if (smem > 40 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewShared) != cudaSuccess) {
+    return fail(GRMX_ERR_LAUNCH, "loss of a few tokens: cannot reserve %d bytes of shared memory: %s", kFewShared, cudaGetErrorString(cudaGetLastError()));
   }
   launch_after(kernel, few_tokens_blocks(V), 1, kFewThreads, smem, s, static_cast<const T*>(hidden), static_cast<const T*>(weight), bias, bias_dtype,
                                                          targets, ignore_index, tokens, D, V, aligned, partials, target_score, ticket);
@@ -308,7 +310,7 @@ int launch_few_tokens(const void* hidden, const void* weight, const void* bias, 
 }
 
 // few enough tokens, and their features fit in shared memory
-bool takes_few_tokens(int64_t N, int64_t D) { return N <= kFewTokens && (D + 511) / 512 * 512 * kFewTokens * 4 <= 160 * 1024; }
+bool takes_few_tokens(int64_t N, int64_t D) { return N <= kFewTokens && (D + 511) / 512 * 512 * kFewTokens * 4 <= kFewShared; }
 
 // ------------------------------------------------------------------ joining the tiles' maxima and sums
 

@@ -11,6 +11,8 @@ above -- over at most 128 + 8 additions between two roundings in full precision,
 bf16 -- and the result is rounded once to its own type.
 """
 
+import threading
+
 import pytest
 import torch
 
@@ -467,3 +469,28 @@ def test_many_tiles_of_short_contractions_and_a_last_one_half_empty(shape):
     for _ in range(30):
         assert all(torch.equal(p, q) for p, q in zip(first, step()))
     cuda_ops.check_device_errors()
+
+
+def test_threads_of_different_widths():
+    # eight tokens of up to 128 KiB of features in shared memory, from two threads at a time
+    inputs = [make(8, D, 64, torch.bfloat16, seed=D) for D in (1536, 2048, 3000, 4096)]
+    wants = [linear_cross_entropy(x, w, t, reduction="none") for x, w, _, t in inputs]
+    failures = []
+
+    def decode(own):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for i in range(3000):
+                    x, w, _, t = inputs[own[i % 2]]
+                    loss = linear_cross_entropy(x, w, t, reduction="none")
+                assert torch.equal(loss, wants[own[1]])
+        except Exception as e:  # noqa: BLE001 -- reported by the test's own thread
+            failures.append(e)
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=decode, args=(own,)) for own in ((0, 3), (1, 2), (2, 0), (3, 1))]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    assert not failures, failures[0]
