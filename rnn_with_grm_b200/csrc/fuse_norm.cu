@@ -339,6 +339,7 @@ __device__ __forceinline__ void stage_params(const RowArgs& a, float* dst, const
   }
 }
 __host__ __device__ constexpr int staged_words(int H) { return H + H / 8 + 1; }
+constexpr int kMostShared = 3 * staged_words(kMaxWidth) * 4;      // of any launch below: the forward pass of the widest row
 
 template <typename T, int VEC, int G, int ACCESS, bool GATE>
 __global__ void __launch_bounds__(threads_of(G), G > 256 ? 1 : 3)
@@ -708,9 +709,10 @@ int64_t most_backward_ctas(int64_t rows, int64_t H) {
 
 template <typename Kernel>
 int launch_rows(Kernel kernel, const RowArgs& a, int64_t grid, int threads, int smem, const char* what, cudaStream_t s) {
-  // (48 KiB without being asked for, less what the kernel holds itself: up to 512 bytes)
-  if (smem > 40 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
-    return fail(GRMX_ERR_LAUNCH, "%s: cannot reserve %d bytes of shared memory: %s", what, smem, cudaGetErrorString(cudaGetLastError()));
+  // (48 KiB without being asked for, less what the kernel holds itself: up to 512 bytes)  Always the same size: a limit of
+  // this call's own could be lowered by another thread's call before the launch below.
+  if (smem > 40 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared) != cudaSuccess) {
+    return fail(GRMX_ERR_LAUNCH, "%s: cannot reserve %d bytes of shared memory: %s", what, kMostShared, cudaGetErrorString(cudaGetLastError()));
   }
   launch_after(kernel, static_cast<unsigned>(grid), 1, threads, smem, s, a);
   return check_launch(what);

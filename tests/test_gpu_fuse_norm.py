@@ -8,6 +8,8 @@ ds by 32 q rstd A (1 + |xh|)^2 taken with the row's largest |xh|, carried throug
 Column sums add the rows' bounds and fp32 additions (a step per row and thread, at most rows + 64 steps of 2^-24).
 """
 
+import threading
+
 import pytest
 import torch
 
@@ -284,3 +286,26 @@ def test_rows_behind_the_last_stay_as_they_are():
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
 def test_parameters_of_about_48_kib(dtype, H):
     check(make(5, H, dtype, True, True, seed=H), with_sum=True)
+
+
+def test_threads_of_different_widths():
+    inputs = [make(4, H, torch.bfloat16, True, True, seed=H) for H in (4105, 5001, 6007, 8001)]      # 54 to 106 KiB
+    wants = [call(t) for t in inputs]
+    failures = []
+
+    def work(own):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for i in range(3000):
+                    out = call(inputs[own[i % 2]])
+                assert torch.equal(out, wants[own[1]])
+        except Exception as e:  # noqa: BLE001 -- reported by the test's own thread
+            failures.append(e)
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(own,)) for own in ((0, 3), (1, 2), (2, 0), (3, 1))]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    assert not failures, failures[0]
