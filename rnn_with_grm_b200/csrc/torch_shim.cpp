@@ -14,6 +14,7 @@
 #include <array>
 #include <atomic>
 #include <cmath>
+#include <initializer_list>
 #include <tuple>
 
 #include "grmx.h"
@@ -781,6 +782,13 @@ at::Tensor or_undefined(const c10::optional<at::Tensor>& t) { return t.has_value
 at::Tensor if_wanted(const at::Tensor& t, bool wanted) { return wanted ? t : at::Tensor(); }
 using MaybeTensor = c10::optional<at::Tensor>;
 
+// neither operator has a forward-mode derivative: a tangent would be lost without a word where no input requires a gradient
+void refuse_tangents(std::initializer_list<const at::Tensor*> inputs, const char* what) {
+  for (const at::Tensor* t : inputs) {
+    TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), what, " has no forward-mode derivative; use reverse mode");
+  }
+}
+
 // gradients with a gradient of their own are asked for (create_graph): they get one that reports its absence
 variable_list no_second_derivative(variable_list grads, const char* what) {
   if (!at::GradMode::is_enabled()) return grads;
@@ -828,6 +836,7 @@ struct LinearCrossEntropyFn : public torch::autograd::Function<LinearCrossEntrop
 at::Tensor linear_cross_entropy(const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& targets,
                                 const c10::optional<at::Tensor>& bias, int64_t ignore_index, int64_t reduction) {
   const at::Tensor b = or_undefined(bias);
+  refuse_tangents({&hidden, &weight, &b}, "linear_cross_entropy");
   if (at::GradMode::is_enabled() && (hidden.requires_grad() || weight.requires_grad() || (b.defined() && b.requires_grad()))) {
     return LinearCrossEntropyFn::apply(hidden, weight, maybe(b), targets, ignore_index, reduction);
   }
@@ -875,6 +884,7 @@ variable_list fuse_layer_norm(const at::Tensor& online, const at::Tensor& update
                               const c10::optional<at::Tensor>& bias, const c10::optional<at::Tensor>& gate,
                               const c10::optional<at::Tensor>& scale, double eps, bool want_sum) {
   const at::Tensor g = or_undefined(gate), k = or_undefined(scale), w = or_undefined(weight), b = or_undefined(bias);
+  refuse_tangents({&online, &update, &w, &b, &g, &k}, "fuse_layer_norm");
   auto needs = [](const at::Tensor& t) { return t.defined() && t.requires_grad(); };
   if (at::GradMode::is_enabled() && (needs(online) || needs(update) || needs(g) || needs(k) || needs(w) || needs(b))) {
     return FuseLayerNormFn::apply(online, update, maybe(g), maybe(k), maybe(w), maybe(b), eps, want_sum);

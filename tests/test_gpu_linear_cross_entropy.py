@@ -494,3 +494,22 @@ def test_threads_of_different_widths():
     for thread in threads:
         thread.join()
     assert not failures, failures[0]
+
+
+def test_forward_mode_and_function_transforms_are_refused():
+    x, w, b, t = make(20, 64, 300, torch.float32, torch.float32, seed=23)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            linear_cross_entropy(dual, w, t, b)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            fuse_layer_norm(dual, x)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            fuse_layer_norm(x, x, gate=dual)
+    linear_cross_entropy(dual, w, t, b)                   # the level is closed: an ordinary tensor again
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda a: linear_cross_entropy(a, w, t[:5]))(x.view(4, 5, 64))
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda a: linear_cross_entropy(a, w, t))(x)
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda a: linear_cross_entropy(a, w, t), (x,), (x,))

@@ -103,3 +103,27 @@ def test_fuse_norm_refuses_row_statistics_off_their_pairs(lib):
         assert lib.grmx_fuse_norm_bwd(some, None, some, some, None, None, None, off, some, some, None, None, None, None, *tail,
                                       None, 0, None) == 1
         assert b"row_stats must be 8-byte aligned" in lib.grmx_last_error()
+
+
+def test_tangents_are_refused_before_anything_else(lib):
+    # (the extension's entry points themselves, which look at tangents before they look at devices)
+    from torch.autograd import forward_ad
+
+    from rnn_with_grm_b200 import cuda_ops
+
+    cuda_ops._require_extension("test")
+    module = cuda_ops._Extension.module
+    x, w, t, v = torch.zeros(4, 8), torch.zeros(10, 8), torch.zeros(4, dtype=torch.long), torch.zeros(8)
+    b = torch.zeros(10)
+    with forward_ad.dual_level():
+        def dual(a):
+            return forward_ad.make_dual(a, torch.ones_like(a))
+
+        for args in ((dual(x), w, t, b), (x, dual(w), t, b), (x, w, t, dual(b))):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                module.linear_cross_entropy(*args, -100, 2)
+        for i in range(6):
+            args = [x, x, v, v, x, v]
+            args[i] = dual(args[i])
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                module.fuse_layer_norm(*args, 1e-5, False)
