@@ -124,6 +124,10 @@ int make_operand(Operand* out, const void* src, int64_t rows, int64_t cols, int 
 
 // ------------------------------------------------------------------ a few tokens
 
+__device__ __forceinline__ float bias_of(const void* bias, int dtype, int64_t word) {
+  return dtype == GRMX_F32 ? static_cast<const float*>(bias)[word] : __bfloat162float(static_cast<const __nv_bfloat16*>(bias)[word]);
+}
+
 // two (maximum, sum of 2^(score - maximum)) pairs into one
 __device__ __forceinline__ float2 join(float2 a, float2 b) {
   const float next = fmaxf(a.x, b.x);
@@ -228,10 +232,7 @@ few_tokens_kernel(const T* __restrict__ hidden, const T* __restrict__ weight, co
   float2 all = make_float2(-INFINITY, 0.0f);
   for (bool loaded = true; v0 < V; v0 += step) {
     const int64_t v = v0 + my_row;
-    float b = 0.0f;
-    if (bias != nullptr && v < V) {
-      b = bias_dtype == GRMX_F32 ? static_cast<const float*>(bias)[v] : __bfloat162float(static_cast<const __nv_bfloat16*>(bias)[v]);
-    }
+    const float b = bias != nullptr && v < V ? bias_of(bias, bias_dtype, v) : 0.0f;
     float acc[M];
 #pragma unroll
     for (int i = 0; i < M; ++i) acc[i] = 0.0f;
@@ -260,7 +261,7 @@ few_tokens_kernel(const T* __restrict__ hidden, const T* __restrict__ weight, co
         }
       }
     }
-    const float y = fmaf(spread_sums<M>(acc, lane), kLog2e, b * kLog2e);
+    const float y = fmaf(spread_sums<M>(acc, lane), kLog2e, bias_base2(b));
     if (v < V) {
       if (v == my_target && lane % kLanesPer == 0) target_score[my_token] = y;
       const float next = fmaxf(all.x, y);
@@ -320,7 +321,7 @@ constexpr int kJoinThreads = 256;
 // added up by the block that finishes last, always in the same order.
 template <int ROWS>
 __global__ void __launch_bounds__(kJoinThreads)
-loss_join_kernel(const float2* __restrict__ partials, const float* __restrict__ target_score,
+loss_join_kernel(const float2* __restrict__ partials, const float* __restrict__ target_score, const void* bias, int bias_dtype,
                  const int64_t* __restrict__ targets, int64_t ignore_index, int64_t vocab, int64_t rows, int parts,
                  int reduction, float* __restrict__ row_max, float* __restrict__ row_sum, float* __restrict__ loss,
                  float* __restrict__ inv_count, double* __restrict__ block_loss, int* __restrict__ block_count,
@@ -365,7 +366,11 @@ loss_join_kernel(const float2* __restrict__ partials, const float* __restrict__ 
     const int64_t t = targets[row];
     if (t != ignore_index) {
       if (t >= 0 && t < vocab) {
-        value = ((mx - target_score[row]) + log2f(sum)) * kLn2;
+        const float below = mx - target_score[row];
+        value = (below + log2f(sum)) * kLn2;
+        // a target masked with the type's lowest value, whose score in base 2 is not the whole of it: beside the mask the
+        // score itself vanishes
+        if (below > 1e38f && bias != nullptr) value = (mx + log2f(sum)) * kLn2 - bias_of(bias, bias_dtype, t);
         counted = 1;
       } else if (error_word != nullptr) {
         atomicOr(error_word, kErrTarget);
@@ -730,7 +735,7 @@ extern "C" int grmx_linear_xent_fwd(const void* hidden, const void* weight, cons
   }
   auto join_kernel = join_rows(N) == 32 ? loss_join_kernel<32> : join_rows(N) == 8 ? loss_join_kernel<8> : loss_join_kernel<1>;
   launch_after(
-      join_kernel, static_cast<unsigned>(f.join_blocks), 1, kJoinThreads, 0, s, partials, target_score, targets, ignore_index, V, N, f.parts, reduction, row_stats, row_stats + N, loss, inv_count,
+      join_kernel, static_cast<unsigned>(f.join_blocks), 1, kJoinThreads, 0, s, partials, target_score, bias, bias_dtype, targets, ignore_index, V, N, f.parts, reduction, row_stats, row_stats + N, loss, inv_count,
       reinterpret_cast<double*>(ws + f.off_loss), reinterpret_cast<int*>(ws + f.off_count), ticket, device_error_word_ptr());
   return check_launch("loss join");
 }

@@ -26,6 +26,8 @@
 // Every wait is bounded; a wait that gives up raises the CTA's and its peer's abort flag, and the error word.
 #pragma once
 
+#include <cfloat>
+
 #include "common.cuh"
 #include "tc_ptx.cuh"
 
@@ -338,6 +340,12 @@ __device__ __forceinline__ float transpose_sum(float (&v)[32], int lane) {
   return v[0];
 }
 
+// A bias in base 2.  A mask of the type's lowest value overflows there; it stays finite (only -inf masks a word for good),
+// so that a row in which nothing else is left has a distribution, equal over its words.
+__device__ __forceinline__ float bias_base2(float b) {
+  const float y = b * kLog2e;
+  return y == -INFINITY && b != -INFINITY ? -FLT_MAX : y;
+}
 // biases of `count` words from word v, base 2, into shared memory; words beyond the vocabulary get -inf
 __device__ __forceinline__ void load_bias(const Params& p, float* dst, int64_t v, int count, int thread, int threads) {
   for (int j = thread; j < count; j += threads) {
@@ -349,7 +357,7 @@ __device__ __forceinline__ void load_bias(const Params& p, float* dst, int64_t v
                                      : __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(p.bias) + v + j));
       }
     }
-    dst[j] = b * kLog2e;
+    dst[j] = bias_base2(b);
   }
 }
 

@@ -27,7 +27,8 @@ def linear_cross_entropy(hidden: Tensor, weight: Tensor, targets: Tensor, bias: 
     float32; gradients come in the types of what they belong to.  ``reduction`` is "none" (``[...]``), "sum" or
     "mean" (over the tokens that count; NaN if none does).  Tokens with ``target == ignore_index`` have loss 0 and
     a zero gradient.  Any other target outside the vocabulary is ignored too and reported by
-    ``cuda_ops.check_device_errors``.  A word whose bias is ``-inf`` is masked: it has probability 0.
+    ``cuda_ops.check_device_errors``.  A word whose bias is ``-inf`` is masked: it has probability 0,
+    and a token without any other word a loss of NaN.  A bias of the type's lowest value is a finite one.
     What the hidden states of ignored tokens hold, NaN included, reaches neither loss nor gradients.
     """
     cuda_ops._require_extension("linear_cross_entropy")

@@ -513,3 +513,39 @@ def test_forward_mode_and_function_transforms_are_refused():
         torch.func.grad(lambda a: linear_cross_entropy(a, w, t))(x)
     with pytest.raises(RuntimeError):
         torch.func.jvp(lambda a: linear_cross_entropy(a, w, t), (x,), (x,))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("N", [5, 40], ids=["few tokens", "tiles"])
+def test_words_masked_with_the_lowest_value(N, dtype):
+    x, w, _, t = make(N, 64, 700, dtype, seed=20)
+    low = torch.finfo(dtype).min
+    b = torch.zeros(700, device=DEV, dtype=dtype)
+    b[256:520] = b[3] = low
+    t = torch.where((t >= 256) & (t < 520) | (t == 3), torch.full_like(t, 100), t)
+    t[2], t[3] = 300, 3                                  # two tokens whose own word is masked
+    leaves = [v.requires_grad_(True) for v in (x, w, b)]
+    loss = linear_cross_entropy(x, w, t, b, reduction="none")
+    grads = torch.autograd.grad(loss, leaves, torch.ones_like(loss))
+    # beside the lowest value the scores vanish: the loss is that value, off by the last bits of fp32 arithmetic
+    masked = torch.zeros(N, dtype=torch.bool, device=DEV)
+    masked[2:4] = True
+    assert ((loss[masked].double() + low).abs() <= 2.0 ** -21 * abs(low)).all()
+    size = torch.where(b == low, torch.zeros_like(b), b)  # (the reference's bounds are of the words that are open)
+    want, tol, want_grads, grad_tols = reference(x, w, torch.where(b == low, torch.full_like(b, float("-inf")), size), t,
+                                                 torch.ones(N, device=DEV))
+    within(loss[~masked], want[~masked], tol[~masked], "loss")
+    for name, grad in zip("xwb", grads):
+        within(grad, want_grads[name], grad_tols[name], "gradient of " + name)
+
+
+@pytest.mark.parametrize("N", [5, 40], ids=["few tokens", "tiles"])
+def test_every_word_masked_with_the_lowest_value(N):
+    # all scores are the lowest value: the words are equally likely
+    x, w, _, t = make(N, 64, 512, torch.float32, seed=21)
+    b = torch.full((512,), torch.finfo(torch.float32).min, device=DEV)
+    leaves = [v.requires_grad_(True) for v in (x, w, b)]
+    loss = linear_cross_entropy(x, w, t, b, reduction="none")
+    assert ((loss.double() - 9 * 0.6931471805599453).abs() <= 2.0 ** -20 * 7).all()
+    for grad in torch.autograd.grad(loss, leaves, torch.ones_like(loss)):
+        assert torch.isfinite(grad).all() and grad.any()
