@@ -83,7 +83,7 @@ struct Params {
   int64_t v0, vocab;
   const void* bias;            // [vocab] or NULL
   int bias_dtype;
-  const int64_t* targets;
+  const int64_t* targets;      // (kEpiStore: of the rows, or NULL)
   int64_t ignore_index;
   // kEpiLse: per row and column tile (times column half in full precision) the maximum and the sum, base 2
   float2* partials;            // [parts][rows]
@@ -626,13 +626,11 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
       if (EPI == kEpiStore) {
         if (p.scale != nullptr) scale = *p.scale;
         if (p.scale2 != nullptr) scale *= *p.scale2;
-        if (p.grad != nullptr && live) {
+        if (p.grad != nullptr && live) scale = __ldg(p.grad + row);
+        if (p.targets != nullptr && live && !isfinite(scale)) {
           // a row that does not count has d = 0 whatever its factor is; 0 x inf must not come of it
-          scale = __ldg(p.grad + row);
-          if (!isfinite(scale)) {
-            const int64_t t = __ldg(p.targets + row);
-            if (t == p.ignore_index || t < 0 || t >= p.vocab) scale = 0.0f;
-          }
+          const int64_t t = __ldg(p.targets + row);
+          if (t == p.ignore_index || t < 0 || t >= p.vocab) scale = 0.0f;
         }
       }
       int target_col = -1;                                   // kEpiLse: the target's column among this group's

@@ -549,3 +549,13 @@ def test_every_word_masked_with_the_lowest_value(N):
     assert ((loss.double() - 9 * 0.6931471805599453).abs() <= 2.0 ** -20 * 7).all()
     for grad in torch.autograd.grad(loss, leaves, torch.ones_like(loss)):
         assert torch.isfinite(grad).all() and grad.any()
+
+
+@pytest.mark.parametrize("reduction", ["sum", "mean"])
+@pytest.mark.parametrize("factor", [float("inf"), float("nan")])
+def test_ignored_tokens_have_no_gradient_whatever_the_factor_is(reduction, factor):
+    x, w, _, t = make(300, 72, 513, torch.bfloat16, ignored=0.3, seed=22)
+    x.requires_grad_(True)
+    loss = linear_cross_entropy(x, w, t, reduction=reduction)
+    (grad,) = torch.autograd.grad(loss, x, torch.tensor(factor, device=DEV))
+    assert not grad[t == -100].any() and not torch.isfinite(grad[t != -100]).any()
