@@ -309,3 +309,60 @@ def test_threads_of_different_widths():
     for thread in threads:
         thread.join()
     assert not failures, failures[0]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("H", [96, 1000, 8184, 8192])
+def test_parameters_off_16_byte_boundaries(dtype, H):
+    # rows that could move whole, beside parameters that cannot
+    t = make(9, H, dtype, True, True, seed=H)
+    for k in ("scale", "weight", "bias"):
+        t[k] = torch.empty(H + 1, device=DEV, dtype=dtype)[1:].copy_(t[k])
+    check(t, with_sum=True)
+
+
+def test_offsets_beyond_32_bits():
+    rows, H = 4_250_000, 512
+    assert rows * H > 1 << 31
+    t = make(rows, H, torch.bfloat16, False, False, seed=10)
+    dy = torch.randn(300, H, device=DEV).bfloat16()
+    ends = [slice(0, 300), slice(rows - 300, rows)]
+    up = torch.zeros(rows, H, device=DEV, dtype=torch.bfloat16)
+    for s in ends:
+        up[s] = dy
+    for k in ("online", "weight"):
+        t[k].requires_grad_(True)
+    y = call(t)
+    d_online, d_weight = torch.autograd.grad(y, [t["online"], t["weight"]], up)
+    total = torch.zeros(H, device=DEV, dtype=torch.float64)
+    for s in ends:
+        part = {k: None if v is None else v.detach()[s] if v.dim() == 2 else v.detach() for k, v in t.items()}
+        want, tol = reference(part, dy, None)
+        within(y[s], want["y"], tol["y"], "y")
+        within(d_online[s], want["online"], tol["online"], "gradient of online")
+        total += want["p_weight"]
+    assert ((d_weight.double() - total).abs() <= 2.0 ** -7 * total.abs() + 1e-3).all()
+    assert not d_online[300:-300].any()
+
+
+def test_wide_rows_off_16_byte_boundaries_in_a_captured_step():
+    t = make(40, 8001, torch.bfloat16, True, True, seed=11)
+    dy = torch.randn(40, 8001, device=DEV).bfloat16()
+    for v in t.values():
+        v.requires_grad_(True)
+
+    def step():
+        y = call(t)
+        return (y.detach(), *torch.autograd.grad(y, list(t.values()), dy))
+
+    want = step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for v in out:
+        v.zero_()
+    call(make(4, 4105, torch.bfloat16, True, True))           # a narrower call in between
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(out, want))

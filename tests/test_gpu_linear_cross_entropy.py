@@ -559,3 +559,103 @@ def test_ignored_tokens_have_no_gradient_whatever_the_factor_is(reduction, facto
     loss = linear_cross_entropy(x, w, t, reduction=reduction)
     (grad,) = torch.autograd.grad(loss, x, torch.tensor(factor, device=DEV))
     assert not grad[t == -100].any() and not torch.isfinite(grad[t != -100]).any()
+
+
+@pytest.mark.parametrize("dtype,shape", [(torch.bfloat16, (2100, 40, 262400)), (torch.bfloat16, (30011, 300, 18300)), (torch.float32, (700, 40, 262400))],
+                         ids=["bf16 cut contraction", "bf16 two column tiles", "fp32 cut contraction"])
+def test_pieces_with_a_factor_per_token(dtype, shape):
+    N, D, V = shape
+    assert 2 * (1 if dtype == torch.bfloat16 else 3) * N * V > 1 << 30       # more than one piece
+    x, w, b, t = make(N, D, V, dtype, torch.float32, ignored=0.1, seed=24)
+    t[0], t[1] = 0, V - 1
+    up = torch.rand(N, device=DEV) + 0.5
+    leaves = [v.requires_grad_(True) for v in (x, w, b)]
+    grads = torch.autograd.grad(linear_cross_entropy(x, w, t, b, reduction="none"), leaves, up)
+    rows = torch.arange(0, N, N // 100, device=DEV)
+    want, _, want_grads, grad_tols = reference(x[rows], w, b, t[rows], up[rows])
+    within(grads[0][rows], want_grads["x"], grad_tols["x"], "gradient of x")
+    X, W, B = x.detach().double(), w.detach().double(), b.detach().double()
+    lse = torch.cat([torch.logsumexp(torch.addmm(B, X[i:i + 500], W.T), 1) for i in range(0, N, 500)])
+    g = torch.where(t != -100, up, torch.zeros_like(up)).double()[:, None]
+    e = (D + 16) * 2.0 ** -23 * (X.abs().sum(1) * W.abs().max() + B.abs().max())
+    for v0 in (0, V // 2 - 60, V - 120):
+        words = torch.arange(v0, v0 + 120, device=DEV)
+        p = torch.exp(X @ W[words].T + B[words] - lse[:, None])
+        unit = p - (t[:, None] == words).double()
+        d = unit * g
+        d_tol = g * (p * (2 * e + 2.0 ** -20)[:, None] * 1.01 + HALF_STEP[dtype] * unit.abs())
+        # drains of 8 blocks in full precision, the whole contraction in bf16; the tokens times their factor are rounded
+        steps = 40 + N * 6 / 512 if dtype == torch.float32 else N + 16
+        tol = (d_tol + (steps * 2.0 ** -23 + HALF_STEP[dtype]) * d.abs()).T @ X.abs() + 2 * HALF_STEP[dtype] * (d.T @ X).abs()
+        within(grads[1][words], d.T @ X, tol, f"gradient of words from {v0}")
+        fine = (d_tol + (40 + N / 32) * 2.0 ** -24 * d.abs()).sum(0)
+        within(grads[2][words], d.sum(0), fine + 2 * HALF_STEP[b.dtype] * d.sum(0).abs(), f"bias gradient of words from {v0}")
+
+
+@pytest.mark.parametrize("shape", [(300, 72, 513), (1500, 300, 5000), (2048, 64, 2048)], ids=lambda s: "x".join(map(str, s)))
+def test_full_precision_sums_are_as_short_as_they_are(shape):
+    """The accumulator is drained every 8 blocks: 32 accumulations and 8 more roundings around them, then one fp32 addition per
+    drain, of which a contraction of `length` has length * 6 / (64 * 8)."""
+    N, D, V = shape
+    x, w, b, t = make(N, D, V, torch.float32, torch.float32, seed=25)
+    leaves = [v.requires_grad_(True) for v in (x, w, b)]
+    grads = torch.autograd.grad(linear_cross_entropy(x, w, t, b, reduction="sum"), leaves)
+    X, W = x.detach().double(), w.detach().double()
+    y = X @ W.T + b.detach().double()
+    e = (D + 16) * 2.0 ** -23 * (X.abs() @ W.abs().T + b.detach().double().abs()).amax(1)
+    p = torch.softmax(y, 1)
+    d = p.scatter_add(1, t[:, None], torch.full((N, 1), -1.0, device=DEV, dtype=torch.float64))
+    d_tol = p * (2 * e + 2.0 ** -20)[:, None] * 1.01 + 2.0 ** -24 * d.abs()
+    for name, grad, a, a_tol, other in (("x", grads[0], d, d_tol, W), ("w", grads[1], d.T, d_tol.T, X)):
+        steps = 40 + len(other) * 6 / 512
+        within(grad, a @ other, (a_tol + steps * 2.0 ** -23 * a.abs()) @ other.abs() + 2.0 ** -23 * (a @ other).abs(), "gradient of " + name)
+
+
+def test_offsets_beyond_32_bits_of_tokens():
+    N, D, V = 4_250_000, 512, 40
+    assert N * D > 1 << 31
+    x, w, b, t = make(N, D, V, torch.bfloat16, torch.float32, ignored=0.1, seed=26)
+    rows = torch.cat([torch.arange(64, device=DEV), torch.arange(N - 300, N, device=DEV)])
+    leaves = [v.requires_grad_(True) for v in (x, b)]
+    loss = linear_cross_entropy(x, w, t, b, reduction="none")
+    dx, db = torch.autograd.grad(loss, leaves, torch.ones_like(loss))
+    want, tol, want_grads, grad_tols = reference(x[rows], w, b, t[rows], torch.ones(len(rows), device=DEV))
+    within(loss[rows], want, tol, "loss")
+    within(dx[rows], want_grads["x"], grad_tols["x"], "gradient of x")
+    assert torch.isfinite(db).all() and not dx[t == -100].any()
+
+
+@pytest.mark.parametrize("N", [3, 16], ids=["few tokens", "tiles"])
+def test_offsets_beyond_32_bits_of_words(N):
+    D, V = 512, 4_250_000
+    assert V * D > 1 << 31
+    x, w, b, t = make(N, D, V, torch.bfloat16, torch.bfloat16, seed=27)
+    t[0], t[1] = V - 1, 4_200_003
+    leaves = [v.requires_grad_(True) for v in (x, w, b)]
+    loss = linear_cross_entropy(x, w, t, b, reduction="none")
+    _, dw, db = torch.autograd.grad(loss, leaves, torch.ones_like(loss))
+    y = torch.cat([x.double() @ w[i:i + 250_000].detach().double().T + b[i:i + 250_000].double() for i in range(0, V, 250_000)], 1).detach()
+    lse = torch.logsumexp(y, 1)
+    e = (D + 16) * 2.0 ** -23 * (x.double().abs().sum(1) * float(w.detach().abs().max()) + float(b.detach().abs().max())).detach()
+    want = lse - y.gather(1, t[:, None])[:, 0]
+    within(loss, want, 2 * e + 2.0 ** -20 * (1 + want.abs()), "loss")
+    words = torch.cat([t, torch.arange(V - 300, V, device=DEV)])
+    unit = torch.exp(y[:, words] - lse[:, None]) - (t[:, None] == words).double()
+    unit_tol = torch.exp(y[:, words] - lse[:, None]) * (2 * e + 2.0 ** -20)[:, None] * 1.01 + 2.0 ** -8 * unit.abs()
+    X = x.detach().double()
+    # (the tokens' factors are ones: nothing is rounded for them)
+    within(dw[words], unit.T @ X, (unit_tol + (N + 16) * 2.0 ** -23 * unit.abs()).T @ X.abs() + 2.0 ** -7 * (unit.T @ X).abs(), "gradient of w")
+    within(db[words], unit.sum(0), (unit_tol + 42 * 2.0 ** -24 * unit.abs()).sum(0) + 2.0 ** -7 * unit.sum(0).abs(), "gradient of b")
+
+
+def test_a_few_wide_tokens_in_a_captured_call():
+    x, w, b, t = make(8, 4096, 300, torch.bfloat16, torch.bfloat16, seed=28)
+    want = linear_cross_entropy(x, w, t, b, reduction="none")
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = linear_cross_entropy(x, w, t, b, reduction="none")
+    out.zero_()
+    linear_cross_entropy(x[:, :2048], w[:, :2048], t, b)      # a narrower call in between
+    graph.replay()
+    assert torch.equal(out, want)
