@@ -719,17 +719,23 @@ int launch_rows(Kernel kernel, const RowArgs& a, int64_t grid, int threads, int 
 }
 
 template <typename T, int VEC, int G, int ACCESS>
+int launch_forward(const RowArgs& a, cudaStream_t s) {
+  constexpr int kGroups = threads_of(G) / G;
+  constexpr int64_t kUnit = kGroups >= 8 ? 1 : 8 / kGroups;
+  int64_t grid = ((a.rows + kGroups - 1) / kGroups + kUnit - 1) / kUnit * kUnit;
+  // a CTA lives for several rows (its set-up costs a fifth of a row of 512)
+  const int64_t most = (G > 256 ? 2 : 6) * static_cast<int64_t>(sm_count()) / kUnit * kUnit;
+  if (grid > most) grid = most;
+  const int smem = ACCESS == kShifted ? 3 * staged_words(a.H) * 4 : 0;
+  return a.gate != nullptr ? launch_rows(fuse_norm_fwd_kernel<T, VEC, G, ACCESS, true>, a, grid, threads_of(G), smem, "fuse_norm", s)
+                           : launch_rows(fuse_norm_fwd_kernel<T, VEC, G, ACCESS, false>, a, grid, threads_of(G), smem, "fuse_norm", s);
+}
+
+template <typename T, int VEC, int G, int ACCESS>
 int launch_group(const RowArgs& a, bool backward, cudaStream_t s) {
   constexpr int kGroups = threads_of(G) / G;
-  if (!backward) {
-    constexpr int64_t kUnit = kGroups >= 8 ? 1 : 8 / kGroups;
-    int64_t grid = ((a.rows + kGroups - 1) / kGroups + kUnit - 1) / kUnit * kUnit;
-    // a CTA lives for several rows (its set-up costs a fifth of a row of 512)
-    const int64_t most = (G > 256 ? 2 : 6) * static_cast<int64_t>(sm_count()) / kUnit * kUnit;
-    if (grid > most) grid = most;
-    const int smem = ACCESS == kShifted ? 3 * staged_words(a.H) * 4 : 0;
-    return a.gate != nullptr ? launch_rows(fuse_norm_fwd_kernel<T, VEC, G, ACCESS, true>, a, grid, threads_of(G), smem, "fuse_norm", s)
-                             : launch_rows(fuse_norm_fwd_kernel<T, VEC, G, ACCESS, false>, a, grid, threads_of(G), smem, "fuse_norm", s);
+  if constexpr (G * kForward <= kMaxWidth) {      // more threads than that no forward pass asks for
+    if (!backward) return launch_forward<T, VEC, G, ACCESS>(a, s);
   }
   const int64_t grid = backward_ctas(a.rows, G);
   const int staged = ACCESS == kShifted ? 2 * staged_words(a.H) * 4 : 0, sums = kGroups > 1 ? kGroups * a.H * 4 : 0;
