@@ -433,7 +433,8 @@ int grmx_archive_push(const float* memory, float* archive, void* archive_bf16, i
  * sum of the scores' exponentials, base 2) and inv_count float32 [1] are what the backward call needs.
  * bf16 products are exact and accumulate in fp32; fp32 inputs are split into three bf16 parts each, of which
  * the six products above 2^-24 are taken.  Masked words (bias -inf) have probability 0; a row without any
- * finite score gives NaN, as does a score of +inf or NaN.  What a token that does not count holds in hidden,
+ * finite score gives NaN, as does a score of +inf or NaN.  A bias of the type's lowest value is finite: where it is all that
+ * a row has, its words are equally likely.  What a token that does not count holds in hidden,
  * NaN included, reaches neither loss nor gradients.
  *
  * workspace: device memory of grmx_linear_xent_workspace(N, D, V, dtype, backward) bytes (0 if N == 0, -1 for
@@ -452,7 +453,9 @@ int grmx_linear_xent_fwd(const void* hidden, const void* weight, const void* bia
  * Gradients of grmx_linear_xent_fwd: grad_loss float32 [N] (GRMX_REDUCE_NONE) or [1]; grad_hidden [N,D] and
  * grad_weight [V,D] in `dtype`, grad_bias [V] in bias_dtype, each of which may be NULL (not wanted).  The scores
  * are computed a second time, in pieces of the vocabulary whose gradients take at most 1 GiB of the workspace
- * (more only where 256 words of all tokens do).  Sums are taken in a fixed order: the same call gives the same
+ * (more only where 256 words of all tokens do).  For bf16 inputs that gradient (without the tokens' factors) is
+ * rounded to bf16 before it is multiplied and added up for grad_bias, and with GRMX_REDUCE_NONE so is hidden times grad_loss
+ * for grad_weight; fp32 inputs have neither rounding.  Sums are taken in a fixed order: the same call gives the same
  * bits.  Every element of the outputs is written.
  */
 int grmx_linear_xent_bwd(const float* grad_loss, const void* hidden, const void* weight, const void* bias,
@@ -472,7 +475,8 @@ int grmx_linear_xent_bwd(const float* grad_loss, const void* hidden, const void*
  * online, update, gate, out, sum_out [rows,H] in `dtype` (GRMX_F32 or GRMX_BF16); scale, ln_weight, ln_bias [H]
  * in param_dtype (GRMX_F32, or dtype), each NULL for the identity; sum_out (s itself, rounded once) may be NULL.
  * row_stats float32 [rows,2] (mean and rstd, what the backward call needs), 8-byte aligned, may be NULL.
- * H <= 8192; arithmetic in fp32.  Rows and parameters on 16-byte boundaries move in 16-byte pieces, others value by value.
+ * H <= 8192; arithmetic in fp32.  Tensors on 16-byte boundaries move in 16-byte pieces whatever H is; if one of the row
+ * tensors starts elsewhere (or H is above 8185 and rows or parameters are off 16-byte boundaries), all move value by value.
  * out may not overlap the inputs.
  *
  * Replaces the residual and gate rules of RetrievedStateFusion with its LayerNorm (grm/core/aggregator.py:116-145)

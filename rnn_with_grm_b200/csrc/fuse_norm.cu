@@ -15,7 +15,9 @@
 // Bound by memory: every row tensor crosses once.  A row belongs to 32 ... 1024 threads, at most 16 values each forward
 // and 8 backward, so that a row, and in the backward pass the column sums of all rows a thread has seen, stay in registers
 // with enough warps resident to cover the loads (backward with 16 values: one CTA per SM, 157 us for 65536 x 512 bf16 against
-// 121 with 8); mean and variance are two passes over those registers.  Row sums are fp32; column sums are fp32 per
+// 121 with 8); mean and variance are two passes over those registers.  Three CTAs per SM leave 80 registers a thread,
+// and the backward pass spills (bytes stored per thread, whole pieces / shifted ones): with gate and scale up to 200 / 336, with
+// one of them 16 / 112 in bf16 and 104 / 104 in fp32; the fp32 forward pass with a gate up to 140.  Row sums are fp32; column sums are fp32 per
 // thread, then joined in a fixed order (groups of a CTA in shared memory, CTAs by a second kernel).
 #include "common.cuh"
 

@@ -85,7 +85,7 @@ struct Params {
   int bias_dtype;
   const int64_t* targets;      // (kEpiStore: of the rows, or NULL)
   int64_t ignore_index;
-  // kEpiLse: per row and column tile (times column half in full precision) the maximum and the sum, base 2
+  // kEpiLse: per row and parts_of() column parts of a tile (two; four in full precision) the maximum and the sum, base 2
   float2* partials;            // [parts][rows]
   float* target_score;         // [rows], base 2
   uint32_t* ticket;            // zeroed for the kernel that follows (or NULL)
@@ -406,8 +406,10 @@ __device__ __forceinline__ void score_gradient(float (&y)[32], const float* bias
   }
 }
 
-// SEG: full precision (six plane products, accumulator drained into registers; both epilogue groups work on
-// every tile).  Otherwise half of the groups work on each accumulator, so on every other tile.
+// SEG: full precision (six plane products, accumulator drained into registers; all four epilogue groups work on
+// every tile, 64 columns each).  Otherwise half of the groups work on each accumulator, so on every other tile.
+// (Registers: the score gradient in full precision spills 196 bytes a thread at the 96 that 18 warps leave, 328 with WEIGHTED;
+// the bf16 forms do not spill.)
 // WEIGHTED (kEpiGrad): the column sums have a factor per row; a kernel of its own, since the plain one is slower by 25 us of
 // 525 with both in it.
 template <int EPI, bool A_MN, bool B_MN, bool SEG, bool WEIGHTED>
@@ -766,7 +768,9 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
             __syncwarp();
             __nv_bfloat16* dst = out + (c / 64) * panel + c % 64 + pl * (p.panels * panel);
             if (!SEG && p.bias_partials != nullptr) {
-              // sums of the rounded values, which is what the weights' gradient is made of as well
+              // Sums of the values as they are stored: they are in the warp's hands there, while sums of the fp32
+              // values take a transposition through 31 shuffles.  The roundings (half a bf16 step of each value, either way)
+              // are those that dW is made of as well, and average out: db is 1.2e-4 off at 2048 ... 16384 tokens.
               const float2 sums = box_out<true, WEIGHTED>(box, dst, 64, rows_here, lane, terms.g);
               if ((lane & 4) == 0) *reinterpret_cast<float2*>(col_sums + c + box_column(lane)) = sums;
             } else {

@@ -28,6 +28,7 @@ def fuse_layer_norm(online: Tensor, update: Tensor, weight: Optional[Tensor] = N
     the vectors ``[H]`` (``scale``, ``weight``, ``bias``, all optional) share a type, that of the rows or float32.
     Arithmetic is float32, results have the type of the rows, gradients that of what they belong to.  With
     ``return_sum`` the result is ``(out, s)``: what the next block adds to, where the norm stands before it.
+    Differentiable once, in reverse mode; inputs with a forward-mode tangent are refused.
     """
     cuda_ops._require_extension("fuse_layer_norm")
     if online.device.type != "cuda":

@@ -21,7 +21,11 @@ _REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 
 def linear_cross_entropy(hidden: Tensor, weight: Tensor, targets: Tensor, bias: Optional[Tensor] = None, *,
                          ignore_index: int = -100, reduction: str = "mean") -> Tensor:
-    """``cross_entropy(hidden @ weight.T + bias, targets)`` in float32, for ``hidden [..., D]`` and ``targets [...]``.
+    """``cross_entropy(hidden @ weight.T + bias, targets)``, for ``hidden [..., D]`` and ``targets [...]``.
+
+    Scores, their exponentials and all sums are float32, and so is the loss.  With bfloat16 inputs the gradient of the
+    scores is rounded to bfloat16 before it is multiplied by ``weight`` and ``hidden`` and added up for ``bias``, and with
+    "none" so are the hidden states times their token's upstream gradient, for the gradient of ``weight``.
 
     ``hidden`` and ``weight [V, D]`` share one type, bfloat16 or float32; ``bias [V]`` has that type or is
     float32; gradients come in the types of what they belong to.  ``reduction`` is "none" (``[...]``), "sum" or
@@ -30,6 +34,7 @@ def linear_cross_entropy(hidden: Tensor, weight: Tensor, targets: Tensor, bias: 
     ``cuda_ops.check_device_errors``.  A word whose bias is ``-inf`` is masked: it has probability 0,
     and a token without any other word a loss of NaN.  A bias of the type's lowest value is a finite one.
     What the hidden states of ignored tokens hold, NaN included, reaches neither loss nor gradients.
+    Differentiable once, in reverse mode; inputs with a forward-mode tangent are refused.
     """
     cuda_ops._require_extension("linear_cross_entropy")
     if reduction not in _REDUCTIONS:
