@@ -366,3 +366,15 @@ def test_wide_rows_off_16_byte_boundaries_in_a_captured_step():
     graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(p, q) for p, q in zip(out, want))
+
+
+def test_equal_gradients_are_two_tensors_of_their_leaves():
+    # without gate and scale one row gradient is written for both
+    t = make(30, 96, torch.bfloat16, False, False, seed=12)
+    for k in ("online", "update"):
+        t[k].requires_grad_(True)
+    call(t).float().square().sum().backward()
+    want = t["update"].grad.clone()
+    assert torch.equal(t["online"].grad, want) and want.any()
+    t["online"].grad.zero_()
+    assert torch.equal(t["update"].grad, want)
